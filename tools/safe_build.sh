@@ -5,11 +5,12 @@
 set -e -o pipefail
 R=$(cd "$(dirname "$0")/.." && pwd)
 OUT=$1; shift
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops"  # as __graft_entry__.build()
 ASM=$(mktemp /tmp/camal_XXXX.s)
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -S --cuda-device-only "$@" -o "$ASM" "$R/camal_amd/csrc/camal_hip.hip" 2>/dev/null
+/opt/rocm/bin/hipcc $FLAGS -S --cuda-device-only "$@" -o "$ASM" "$R/camal_amd/csrc/camal_hip.hip" 2>/dev/null
 if ! python3 "$R/tools/check_ring.py" "$ASM" | tail -3; then
   echo "ring checker: findings -- not building $OUT"; rm -f "$ASM"; exit 1
 fi
 rm -f "$ASM"
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared "$@" -o "$OUT" "$R/camal_amd/csrc/camal_hip.hip"
+/opt/rocm/bin/hipcc $FLAGS -fPIC -shared "$@" -o "$OUT" "$R/camal_amd/csrc/camal_hip.hip"
 echo "built $OUT"

@@ -5,7 +5,7 @@ Public surface mirrors the reference (adrienpetralia/CamAL):
 Everything heavy is imported lazily so that ``import camal_amd`` works without a GPU.
 """
 __all__ = ["CamAL", "CamALResNet", "ResNet", "CAM", "Ensemble", "NILMmetrics", "Classifmetrics", "BasedClassifTrainer", "TSLoader",
-           "TSDataset", "NILMscaler"]
+           "TSDataset", "NILMscaler", "ActivationCheckpoint"]
 
 
 def __getattr__(name):
@@ -33,4 +33,7 @@ def __getattr__(name):
     if name == "NILMscaler":
         from .windows import NILMscaler
         return NILMscaler
+    if name == "ActivationCheckpoint":
+        from .act_checkpoint import ActivationCheckpoint
+        return ActivationCheckpoint
     raise AttributeError(name)

@@ -13,6 +13,7 @@ LIB_PATH = os.environ.get("CAMAL_HIP_LIB") or os.path.join(_HERE, "libcamal_hip.
 
 ARCH_CAMAL, ARCH_RESNET = 0, 1
 FP32, BF16 = 0, 1
+ACT_INT8, ACT_E4M3 = 0, 1
 PROF_CLASSES = ("stem", "conv", "conv_cam_head", "post", "other")
 
 
@@ -65,6 +66,12 @@ SIGNATURES = {
     "camal_train_fwd_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, C.c_float, _vp, _vp, _vp, _vp, _vp]),
     "camal_trainer_peek": (_i, [_vp, _i, _i, _i, _i, _vp, _sz, C.POINTER(_i), _vp]),
     "camal_train_bwd_dlogits": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp]),
+    "camal_act_write": (_i, [_vp] * 5 + [_i] + [_vp] * 5 + [C.c_longlong, _i, _i] + [_vp] * 6),
+    "camal_act_read": (_i, [_vp, _vp, _i, C.c_longlong, _i, _vp, _vp, _i] + [_vp] * 6),
+    "camal_act_norm_bwd_workspace_bytes": (_sz, [C.c_longlong, _i]),
+    "camal_act_norm_bwd": (_i, [_vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "camal_act_wgrad_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "camal_act_wgrad": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _sz, _vp]),
     "camal_ce_eval": (_i, [_vp, _vp, _i, _vp, _vp, _vp]),
     "camal_adamw_step": (_i, [_vp, _vp, _vp, _vp, _sz, _i, C.c_float, C.c_float, C.c_float, C.c_float, C.c_float, _vp]),
     "camal_set_profiling": (_i, [_vp, _i]),

@@ -1,0 +1,220 @@
+// camal_act_impl.hpp — host side of the 8-bit activation checkpoints (included by camal_hip.hip): argument checks, launch
+// shapes and the camal_act_* entry points.
+#pragma once
+#include <climits>
+
+#include "camal_act_kernels.hpp"
+
+namespace {
+
+inline bool act_channels_ok(int c) { return c == 32 || c == 64 || c == 128 || c == 256; }
+inline bool act_aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+inline bool act_format_ok(int f) { return f == CAMAL_ACT_INT8 || f == CAMAL_ACT_E4M3; }
+
+// Calls f(format type); every entry point checks the format first
+template <typename Fn>
+int act_dispatch(int format, Fn&& f) {
+    return format == CAMAL_ACT_INT8 ? f(ActI8()) : f(ActE4M3());
+}
+template <typename Fn>
+int act_dispatch_c(int c, Fn&& f) {
+    switch (c) {
+        case 32: return f(std::integral_constant<int, 32>());
+        case 64: return f(std::integral_constant<int, 64>());
+        case 128: return f(std::integral_constant<int, 128>());
+        case 256: return f(std::integral_constant<int, 256>());
+    }
+    return fail(CAMAL_ERR_ARG, "channels must be 32, 64, 128 or 256");
+}
+
+// What the entry points share: null pointers, alignment of the float rows (16-byte loads) and of the codes (4-byte loads)
+int act_check(std::initializer_list<const void*> floats, std::initializer_list<const void*> codes,
+              std::initializer_list<const void*> bytes, long long rows, int channels, int format) {
+    if (rows < 1 || rows > INT_MAX) return fail(CAMAL_ERR_ARG, "the number of rows must be in 1 .. 2^31 - 1");
+    if (!act_channels_ok(channels)) return fail(CAMAL_ERR_ARG, "channels must be 32, 64, 128 or 256");
+    if (!act_format_ok(format)) return fail(CAMAL_ERR_ARG, "format must be CAMAL_ACT_INT8 or CAMAL_ACT_E4M3");
+    for (const void* p : floats) {
+        if (!p) return fail(CAMAL_ERR_ARG, "null argument");
+        if (!act_aligned(p, 16)) return fail(CAMAL_ERR_ARG, "float tensors must be 16-byte aligned");
+    }
+    for (const void* p : codes) {
+        if (!p) return fail(CAMAL_ERR_ARG, "null argument");
+        if (!act_aligned(p, 4)) return fail(CAMAL_ERR_ARG, "codes must be 4-byte aligned");
+    }
+    for (const void* p : bytes)
+        if (!p) return fail(CAMAL_ERR_ARG, "null argument");
+    return 0;
+}
+
+inline int act_blocks(size_t work, size_t per_block, int cap) { return (int)std::min<size_t>((work + per_block - 1) / per_block, (size_t)cap); }
+
+template <typename F, bool RELU, bool RES>
+int act_write(hipStream_t s, const float* z, ActNorm n, const float* zr, ActNorm nr, size_t rows, int channels, float* out,
+              void* codes, unsigned char* scales, void* codes_r, unsigned char* scales_r) {
+    const size_t n4 = rows * (size_t)(channels / 4);
+    hipLaunchKernelGGL((act_write_kernel<F, RELU, RES>), dim3(act_blocks(n4, 256 * ACT_ROWS, 4096)), dim3(256), 0, s, z, n, zr, nr,
+                       out, (unsigned*)codes, scales, (unsigned*)codes_r, scales_r, n4, channels / 4 - 1);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+template <typename F, bool AFFINE, bool RELU, bool RES>
+int act_read(hipStream_t s, const ActIn& in, size_t rows, int channels, float* out) {
+    const size_t n4 = rows * (size_t)(channels / 4);
+    hipLaunchKernelGGL((act_read_kernel<F, AFFINE, RELU, RES>), dim3(act_blocks(n4, 256, 4096)), dim3(256), 0, s, in.codes,
+                       in.scales, in.gamma, in.beta, in.codes_r, in.scales_r, in.gamma_r, in.beta_r, out, n4, channels / 4 - 1);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+inline size_t act_bwd_blocks(size_t rows) { return (rows + BN_ROWS_PER_BLOCK - 1) / BN_ROWS_PER_BLOCK; }
+// workspace of the norm backward: partial sums [blocks][channels][2] in 64 bits, then the two rows of means
+inline size_t act_bwd_bytes(size_t rows, int channels) {
+    return act_bwd_blocks(rows) * channels * 2 * sizeof(double) + 2 * (size_t)channels * sizeof(float);
+}
+
+template <typename F, int C, bool RELU, bool BCAST>
+int act_norm_bwd(hipStream_t s, const float* da, const void* codes, const unsigned char* scales, const float* invstd,
+                 const float* gamma, const float* beta, int N, int L, float* dz, float* dgamma, float* dbeta, void* ws) {
+    const int nb = (int)act_bwd_blocks(N);
+    double* partial = (double*)ws;
+    float* means = (float*)(partial + (size_t)nb * C * 2);
+    const size_t n4 = (size_t)N * (C / 4);
+    hipLaunchKernelGGL((act_bwd_partial_kernel<F, C, RELU, BCAST>), dim3(nb), dim3(256), 0, s, da, (const unsigned*)codes, scales,
+                       gamma, beta, N, L, partial);
+    hipLaunchKernelGGL(act_bwd_final_kernel<C>, dim3(C / BN_FINAL_CPB), dim3(BN_FINAL_THREADS), 0, s, partial, nb, N, means,
+                       dgamma, dbeta);
+    hipLaunchKernelGGL((act_bwd_apply_kernel<F, C, RELU, BCAST>), dim3(act_blocks(n4, 256, 4096)), dim3(256), 0, s, da,
+                       (const unsigned*)codes, scales, invstd, gamma, beta, means, n4, L, dz);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+// Splits of the batch of the weight gradient, fixed by the shapes alone: the sums have the same order on every call
+struct ActSplits { int nsplit, tiles; };
+ActSplits act_wgrad_splits(int B, int L, int cin, int cout, int ks) {
+    const int total = B * ((L + ACT_WG_TT - 1) / ACT_WG_TT);
+    const int want = std::min(std::max(1, 2048 / ((cin / 32) * (cout / 32) * ks)), total);
+    const int tiles = (total + want - 1) / want;
+    return {(total + tiles - 1) / tiles, tiles};
+}
+
+template <typename F, bool RELU, bool RES>
+int act_wgrad(hipStream_t s, const float* dz, const ActIn& in, int B, int L, int cin, int cout, int ks, bool zero_pad, float* dw,
+              float* bias_grad, float* part) {
+    const ActSplits sp = act_wgrad_splits(B, L, cin, cout, ks);
+    hipLaunchKernelGGL((act_wgrad_simple_kernel<F, RELU, RES>), dim3(sp.nsplit, (cin / 32) * (cout / 32), ks), dim3(256), 0, s, dz,
+                       in, part, B, L, cin, cout, ks, sp.tiles, zero_pad);
+    const int total = cout * cin * ks;
+    hipLaunchKernelGGL(wgrad_reduce_kernel, dim3((total / 4 + 63) / 64), dim3(256), 0, s, part, sp.nsplit, cout, cin, ks, dw,
+                       bias_grad);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int camal_act_write(const float* z, const float* mean, const float* invstd, const float* gamma, const float* beta, int relu,
+                    const float* zr, const float* mean_r, const float* invstd_r, const float* gamma_r, const float* beta_r,
+                    long long rows, int channels, int format, float* out, void* codes, unsigned char* scales, void* codes_r,
+                    unsigned char* scales_r, void* stream) {
+    if (int r = act_check({z, mean, invstd, gamma, beta, out}, {codes}, {scales}, rows, channels, format)) return r;
+    if (zr)
+        if (int r = act_check({mean_r, invstd_r, gamma_r, beta_r, zr}, {codes_r}, {scales_r}, rows, channels, format)) return r;
+    const ActNorm n{mean, invstd, gamma, beta}, nr{mean_r, invstd_r, gamma_r, beta_r};
+    hipStream_t s = (hipStream_t)stream;
+    return act_dispatch(format, [&](auto f) {
+        using F = decltype(f);
+        if (zr)
+            return relu ? act_write<F, true, true>(s, z, n, zr, nr, rows, channels, out, codes, scales, codes_r, scales_r)
+                        : act_write<F, false, true>(s, z, n, zr, nr, rows, channels, out, codes, scales, codes_r, scales_r);
+        return relu ? act_write<F, true, false>(s, z, n, zr, nr, rows, channels, out, codes, scales, codes_r, scales_r)
+                    : act_write<F, false, false>(s, z, n, zr, nr, rows, channels, out, codes, scales, codes_r, scales_r);
+    });
+}
+
+int camal_act_read(const void* codes, const unsigned char* scales, int format, long long rows, int channels, const float* gamma,
+                   const float* beta, int relu, const void* codes_r, const unsigned char* scales_r, const float* gamma_r,
+                   const float* beta_r, float* out, void* stream) {
+    if (int r = act_check({out}, {codes}, {scales}, rows, channels, format)) return r;
+    if ((gamma != nullptr) != (beta != nullptr)) return fail(CAMAL_ERR_ARG, "gamma and beta come together");
+    if (!gamma && (relu || codes_r)) return fail(CAMAL_ERR_ARG, "the activation needs gamma and beta");
+    if (gamma)
+        if (int r = act_check({gamma, beta}, {}, {}, rows, channels, format)) return r;
+    if (codes_r)
+        if (int r = act_check({gamma_r, beta_r}, {codes_r}, {scales_r}, rows, channels, format)) return r;
+    const ActIn in{(const unsigned*)codes, scales, gamma, beta, (const unsigned*)codes_r, scales_r, gamma_r, beta_r};
+    hipStream_t s = (hipStream_t)stream;
+    return act_dispatch(format, [&](auto f) {
+        using F = decltype(f);
+        if (!gamma) return act_read<F, false, false, false>(s, in, rows, channels, out);
+        if (codes_r)
+            return relu ? act_read<F, true, true, true>(s, in, rows, channels, out) : act_read<F, true, false, true>(s, in, rows, channels, out);
+        return relu ? act_read<F, true, true, false>(s, in, rows, channels, out) : act_read<F, true, false, false>(s, in, rows, channels, out);
+    });
+}
+
+size_t camal_act_norm_bwd_workspace_bytes(long long rows, int channels) {
+    return rows < 1 || rows > INT_MAX || !act_channels_ok(channels) ? 0 : act_bwd_bytes((size_t)rows, channels);
+}
+
+int camal_act_norm_bwd(const float* da, int pooled, const void* codes, const unsigned char* scales, int format, int B, int L,
+                       int channels, const float* invstd, const float* gamma, const float* beta, int relu, float* dz,
+                       float* dgamma, float* dbeta, void* workspace, size_t workspace_bytes, void* stream) {
+    if (B < 1 || L < 1) return fail(CAMAL_ERR_ARG, "B and L must be >= 1");
+    const long long rows = (long long)B * L;
+    if (int r = act_check({da, invstd, gamma, beta, dz, workspace}, {codes, dgamma, dbeta}, {scales}, rows, channels, format)) return r;
+    if (workspace_bytes < act_bwd_bytes((size_t)rows, channels))
+        return fail(CAMAL_ERR_ARG, "workspace smaller than camal_act_norm_bwd_workspace_bytes(B * L, channels)");
+    hipStream_t s = (hipStream_t)stream;
+    return act_dispatch(format, [&](auto f) {
+        using F = decltype(f);
+        return act_dispatch_c(channels, [&](auto c) {
+            constexpr int C = decltype(c)::value;
+            const int N = (int)rows;
+            if (pooled)
+                return relu ? act_norm_bwd<F, C, true, true>(s, da, codes, scales, invstd, gamma, beta, N, L, dz, dgamma, dbeta, workspace)
+                            : act_norm_bwd<F, C, false, true>(s, da, codes, scales, invstd, gamma, beta, N, L, dz, dgamma, dbeta, workspace);
+            return relu ? act_norm_bwd<F, C, true, false>(s, da, codes, scales, invstd, gamma, beta, N, L, dz, dgamma, dbeta, workspace)
+                        : act_norm_bwd<F, C, false, false>(s, da, codes, scales, invstd, gamma, beta, N, L, dz, dgamma, dbeta, workspace);
+        });
+    });
+}
+
+static bool act_wgrad_shape_ok(int B, int L, int cin, int cout, int ks) {
+    return B >= 1 && L >= 1 && (long long)B * L <= INT_MAX && act_channels_ok(cin) && act_channels_ok(cout) && ks >= 1 && ks <= 63 && (ks & 1);
+}
+
+size_t camal_act_wgrad_workspace_bytes(int B, int L, int cin, int cout, int ks) {
+    if (!act_wgrad_shape_ok(B, L, cin, cout, ks)) return 0;
+    return (size_t)act_wgrad_splits(B, L, cin, cout, ks).nsplit * ks * cout * cin * sizeof(float);
+}
+
+int camal_act_wgrad(const float* dz, const void* codes, const unsigned char* scales, int format, int B, int L, int cin, int cout,
+                    int ks, const float* gamma, const float* beta, int relu, const void* codes_r, const unsigned char* scales_r,
+                    const float* gamma_r, const float* beta_r, int zero_pad, float* dw, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+    if (!act_wgrad_shape_ok(B, L, cin, cout, ks))
+        return fail(CAMAL_ERR_ARG, "B, L >= 1, cin and cout in {32, 64, 128, 256}, ks odd and in 1..63");
+    const long long rows = (long long)B * L;
+    if (int r = act_check({dz, gamma, beta, workspace}, {codes, dw}, {scales}, rows, cin, format)) return r;
+    if (codes_r)
+        if (int r = act_check({gamma_r, beta_r}, {codes_r}, {scales_r}, rows, cin, format)) return r;
+    if (workspace_bytes < camal_act_wgrad_workspace_bytes(B, L, cin, cout, ks))
+        return fail(CAMAL_ERR_ARG, "workspace smaller than camal_act_wgrad_workspace_bytes(B, L, cin, cout, ks)");
+    const ActIn in{(const unsigned*)codes, scales, gamma, beta, (const unsigned*)codes_r, scales_r, gamma_r, beta_r};
+    hipStream_t s = (hipStream_t)stream;
+    float* part = (float*)workspace;
+    return act_dispatch(format, [&](auto f) {
+        using F = decltype(f);
+        if (codes_r)
+            return relu ? act_wgrad<F, true, true>(s, dz, in, B, L, cin, cout, ks, zero_pad != 0, dw, nullptr, part)
+                        : act_wgrad<F, false, true>(s, dz, in, B, L, cin, cout, ks, zero_pad != 0, dw, nullptr, part);
+        return relu ? act_wgrad<F, true, false>(s, dz, in, B, L, cin, cout, ks, zero_pad != 0, dw, nullptr, part)
+                    : act_wgrad<F, false, false>(s, dz, in, B, L, cin, cout, ks, zero_pad != 0, dw, nullptr, part);
+    });
+}
+
+}  // extern "C"

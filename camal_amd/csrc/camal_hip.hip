@@ -1262,4 +1262,5 @@ int camal_get_profile(camal_ctx* c, int* launches, double* ms) {
 
 }  // extern "C"
 
+#include "camal_act_impl.hpp"
 #include "camal_train_impl.hpp"

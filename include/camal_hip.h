@@ -304,6 +304,64 @@ int camal_train_bwd_dlogits(camal_trainer* t, const float* params_dev, const flo
 int camal_trainer_peek(camal_trainer* t, int what, int index, int B, int L, float* out_dev, size_t out_floats,
                        int* channels_out, void* stream);
 
+/* ------------------------------- 8-bit activation checkpoints -------------------------------
+ * What a training step keeps of its forward pass for its backward pass, at 1.03 bytes per element instead of 8 (the
+ * fp32 convolution output and the fp32 activation behind it).  No counterpart in the reference, whose autograd keeps
+ * both in fp32 (torch_trainer.py:288-291).  Tensors are [window][time][channel]; a "row" is one timestep of one window.
+ *
+ * A checkpoint is codes [rows][channels], one byte each, and scales [rows][channels / 32], one byte per block of 32
+ * consecutive channels.  It holds the normalised value x = fl(fl(z - mean) * invstd) of a train-mode BatchNorm as
+ * code * 2^(scale - 127):
+ *   CAMAL_ACT_INT8  code = two's complement byte, the scale is the smallest power of two with max|x| <= 127 * 2^(scale-127)
+ *   CAMAL_ACT_E4M3  code = OCP e4m3 (4 exponent, 3 fraction bits), max|x| <= 448 * 2^(scale-127)
+ * (scale >= 1; 255 with zero codes = the block holds an infinity, a NaN or a magnitude over 127 * 2^121 (int8) or
+ * 448 * 2^119 (e4m3): it reads back as NaN).  x is rounded to the nearest code, ties to even.  With relu, where that code would put fma(value, gamma, beta) on the other side of the
+ * ReLU than fma(x, gamma, beta), the neighbour on x's side is taken: the backward pass has the forward pass's mask
+ * exactly (gamma and beta must be the ones the checkpoint was written with).
+ *
+ * channels in {32, 64, 128, 256}; 1 <= rows < 2^31.  float tensors 16-byte aligned, codes 4-byte aligned; inputs and
+ * outputs must not overlap.  All calls are asynchronous on `stream`, on the current device, allocate nothing and may be
+ * captured into a graph; results do not depend on scheduling.  Calls that can overlap need workspaces of their own. */
+#define CAMAL_ACT_INT8 0
+#define CAMAL_ACT_E4M3 1
+
+/* Normalise, ReLU (relu != 0), add the skip branch, and keep:
+ *   out_dev = [relu](fma(x, gamma, beta)) [+ fma(x_r, gamma_r, beta_r)]  fp32 [rows][channels], and the checkpoint(s) of
+ * x (and of x_r, which has no ReLU).  z_dev, zr_dev: fp32 convolution outputs; zr_dev NULL: no skip branch (the
+ * arguments that end in _r are then not looked at).  mean, invstd: batch statistics [channels].                   */
+int camal_act_write(const float* z_dev, const float* mean, const float* invstd, const float* gamma, const float* beta, int relu,
+                    const float* zr_dev, const float* mean_r, const float* invstd_r, const float* gamma_r, const float* beta_r,
+                    long long rows, int channels, int format, float* out_dev, void* codes_dev, unsigned char* scales_dev,
+                    void* codes_r_dev, unsigned char* scales_r_dev, void* stream);
+
+/* Read a checkpoint back into out_dev [rows][channels] fp32: the normalised values (gamma and beta NULL), or the
+ * activation [relu](fma(x, gamma, beta)) [+ fma(x_r, gamma_r, beta_r)] (codes_r_dev NULL: no skip branch).          */
+int camal_act_read(const void* codes_dev, const unsigned char* scales_dev, int format, long long rows, int channels,
+                   const float* gamma, const float* beta, int relu, const void* codes_r_dev, const unsigned char* scales_r_dev,
+                   const float* gamma_r, const float* beta_r, float* out_dev, void* stream);
+
+/* Backward of BatchNorm (+ ReLU) from the checkpoint, N = B * L rows:
+ *   dy = da * [fma(x, gamma, beta) > 0] (relu != 0; else dy = da),  dbeta = sum dy,  dgamma = sum dy x,
+ *   dz = gamma invstd (dy - dbeta / N - x dgamma / N)
+ * da_dev [B][L][channels], or with pooled != 0 [B][channels], the gradient of each window's mean over time: every
+ * timestep gets da / L.  Sums are held in 64 bits across workgroups.                                              */
+size_t camal_act_norm_bwd_workspace_bytes(long long rows, int channels); /* 0 if unsupported */
+int camal_act_norm_bwd(const float* da_dev, int pooled, const void* codes_dev, const unsigned char* scales_dev, int format, int B,
+                       int L, int channels, const float* invstd, const float* gamma, const float* beta, int relu, float* dz_dev,
+                       float* dgamma, float* dbeta, void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* Weight gradient of a Conv1d (odd ks; ks = 1: a linear layer) whose input is held as checkpoint(s):
+ *   dw[co][ci][j] = sum_{b,t} dz[b][t][co] * a[b][clamp(t + j - ks/2, 0, L-1)][ci]      (zero_pad: 0 outside the window)
+ *   a = bf16([relu](fma(x, gamma, beta)) [+ fma(x_r, gamma_r, beta_r)])
+ * The activation enters with the 8 significant bits of bf16 (its code has at most 7); dz enters with all of its 24 and
+ * the products are summed in fp32.  dz_dev [B][L][cout] fp32, dw [cout][cin][ks] fp32.  cin, cout in {32, 64, 128, 256},
+ * ks <= 63.  An infinite dz gives NaN.                                                                             */
+size_t camal_act_wgrad_workspace_bytes(int B, int L, int cin, int cout, int ks); /* 0 if unsupported */
+int camal_act_wgrad(const float* dz_dev, const void* codes_dev, const unsigned char* scales_dev, int format, int B, int L, int cin,
+                    int cout, int ks, const float* gamma, const float* beta, int relu, const void* codes_r_dev,
+                    const unsigned char* scales_r_dev, const float* gamma_r, const float* beta_r, int zero_pad, float* dw,
+                    void* workspace_dev, size_t workspace_bytes, void* stream);
+
 /* Evaluation loss of BasedClassifTrainer.evaluate / __evaluate (torch_trainer.py:188-193,316-321) from eval-mode
  * logits (camal_forward_cam): per-window cross-entropy (float32, -log_softmax[label]) and predicted label (argmax,
  * the first maximum like torch.max).  logits_dev [B][2] float32, labels_dev [B] int32, loss_out [B] float32,

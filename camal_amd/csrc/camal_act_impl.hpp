@@ -90,23 +90,46 @@ int act_norm_bwd(hipStream_t s, const float* da, const void* codes, const unsign
     return 0;
 }
 
-// Splits of the batch of the weight gradient, fixed by the shapes alone: the sums have the same order on every call
-struct ActSplits { int nsplit, tiles; };
-ActSplits act_wgrad_splits(int B, int L, int cin, int cout, int ks) {
-    const int total = B * ((L + ACT_WG_TT - 1) / ACT_WG_TT);
-    const int want = std::min(std::max(1, 2048 / ((cin / 32) * (cout / 32) * ks)), total);
-    const int tiles = (total + want - 1) / want;
-    return {(total + tiles - 1) / tiles, tiles};
+// How the weight gradient is cut up, fixed by the shapes alone: the sums have the same order on every call.
+// Tap groups of nearly equal size (9 = 5 + 4, 25 = 7 + 6 + 6 + 6); CIW = 32-wide ci tiles per wave: two where few taps leave
+// room for the accumulators, so that the pieces of dz serve more products; splits for two workgroups on each of 256 CUs.
+struct ActPlan { int B, L, ciw, wk, groups, n_hi, nhi, nsplit, units; };
+ActPlan act_wgrad_plan(int B, int L, int cin, int cout, int ks) {
+    ActPlan p;
+    p.B = ks == 1 ? 1 : B;  // one tap knows no window edges
+    p.L = ks == 1 ? B * L : L;
+    p.groups = (ks + ACT_TAPS - 1) / ACT_TAPS;
+    const int base = ks / p.groups, rem = ks % p.groups;
+    p.nhi = rem ? base + 1 : base;
+    p.n_hi = rem ? rem : p.groups;
+    p.ciw = cin >= 64 && p.nhi <= 4 ? 2 : 1;
+    p.wk = cout >= 128 ? 1 : 128 / cout;
+    const int total = p.B * ((p.L + ACT_UNIT - 1) / ACT_UNIT), iters = (total + p.wk - 1) / p.wk;
+    const int want = std::min(std::max(1, 512 / (p.groups * (cin / (32 * p.ciw)) * std::max(1, cout / 128))), iters);
+    p.units = (iters + want - 1) / want * p.wk;
+    p.nsplit = (total + p.units - 1) / p.units;
+    return p;
 }
 
-template <typename F, bool RELU, bool RES>
-int act_wgrad(hipStream_t s, const float* dz, const ActIn& in, int B, int L, int cin, int cout, int ks, bool zero_pad, float* dw,
+int act_wgrad(hipStream_t s, const float* dz, const ActIn& in, int B, int L, int cin, int cout, int ks, float* dw,
               float* bias_grad, float* part) {
-    const ActSplits sp = act_wgrad_splits(B, L, cin, cout, ks);
-    hipLaunchKernelGGL((act_wgrad_simple_kernel<F, RELU, RES>), dim3(sp.nsplit, (cin / 32) * (cout / 32), ks), dim3(256), 0, s, dz,
-                       in, part, B, L, cin, cout, ks, sp.tiles, zero_pad);
+    const ActPlan p = act_wgrad_plan(B, L, cin, cout, ks);
+    const dim3 grid(p.nsplit, p.groups * (cin / (32 * p.ciw)), std::max(1, cout / 128));
+    auto launch = [&](auto co, auto ciw, auto nt) {
+        hipLaunchKernelGGL((act_wgrad_kernel<decltype(co)::value, decltype(ciw)::value, decltype(nt)::value>), grid, dim3(256), 0, s, dz,
+                           in, part, p.B, p.L, cin, ks, p.units, p.n_hi);
+        return 0;
+    };
+    const int rc = act_dispatch_c(cout, [&](auto co) {
+#define CAMAL_ACT_WG(W, N) if (p.ciw == W && p.nhi == N) return launch(co, std::integral_constant<int, W>(), std::integral_constant<int, N>());
+        CAMAL_ACT_WG(1, 1) CAMAL_ACT_WG(1, 3) CAMAL_ACT_WG(1, 5) CAMAL_ACT_WG(1, 6) CAMAL_ACT_WG(1, 7) CAMAL_ACT_WG(1, 8)
+        CAMAL_ACT_WG(2, 1) CAMAL_ACT_WG(2, 3)
+#undef CAMAL_ACT_WG
+        return fail(CAMAL_ERR_STATE, "no weight-gradient kernel for this kernel size");
+    });
+    if (rc) return rc;
     const int total = cout * cin * ks;
-    hipLaunchKernelGGL(wgrad_reduce_kernel, dim3((total / 4 + 63) / 64), dim3(256), 0, s, part, sp.nsplit, cout, cin, ks, dw,
+    hipLaunchKernelGGL(wgrad_reduce_kernel, dim3((total / 4 + 63) / 64), dim3(256), 0, s, part, p.nsplit * p.wk, cout, cin, ks, dw,
                        bias_grad);
     HIP_TRY(hipGetLastError());
     return 0;
@@ -145,7 +168,7 @@ int camal_act_read(const void* codes, const unsigned char* scales, int format, l
         if (int r = act_check({gamma, beta}, {}, {}, rows, channels, format)) return r;
     if (codes_r)
         if (int r = act_check({gamma_r, beta_r}, {codes_r}, {scales_r}, rows, channels, format)) return r;
-    const ActIn in{(const unsigned*)codes, scales, gamma, beta, (const unsigned*)codes_r, scales_r, gamma_r, beta_r};
+    const ActIn in{(const unsigned*)codes, scales, gamma, beta, (const unsigned*)codes_r, scales_r, gamma_r, beta_r, 0, 0, 0};
     hipStream_t s = (hipStream_t)stream;
     return act_dispatch(format, [&](auto f) {
         using F = decltype(f);
@@ -189,7 +212,8 @@ static bool act_wgrad_shape_ok(int B, int L, int cin, int cout, int ks) {
 
 size_t camal_act_wgrad_workspace_bytes(int B, int L, int cin, int cout, int ks) {
     if (!act_wgrad_shape_ok(B, L, cin, cout, ks)) return 0;
-    return (size_t)act_wgrad_splits(B, L, cin, cout, ks).nsplit * ks * cout * cin * sizeof(float);
+    const ActPlan p = act_wgrad_plan(B, L, cin, cout, ks);
+    return (size_t)p.nsplit * p.wk * ks * cout * cin * sizeof(float);
 }
 
 int camal_act_wgrad(const float* dz, const void* codes, const unsigned char* scales, int format, int B, int L, int cin, int cout,
@@ -204,17 +228,9 @@ int camal_act_wgrad(const float* dz, const void* codes, const unsigned char* sca
         if (int r = act_check({gamma_r, beta_r}, {codes_r}, {scales_r}, rows, cin, format)) return r;
     if (workspace_bytes < camal_act_wgrad_workspace_bytes(B, L, cin, cout, ks))
         return fail(CAMAL_ERR_ARG, "workspace smaller than camal_act_wgrad_workspace_bytes(B, L, cin, cout, ks)");
-    const ActIn in{(const unsigned*)codes, scales, gamma, beta, (const unsigned*)codes_r, scales_r, gamma_r, beta_r};
-    hipStream_t s = (hipStream_t)stream;
-    float* part = (float*)workspace;
-    return act_dispatch(format, [&](auto f) {
-        using F = decltype(f);
-        if (codes_r)
-            return relu ? act_wgrad<F, true, true>(s, dz, in, B, L, cin, cout, ks, zero_pad != 0, dw, nullptr, part)
-                        : act_wgrad<F, false, true>(s, dz, in, B, L, cin, cout, ks, zero_pad != 0, dw, nullptr, part);
-        return relu ? act_wgrad<F, true, false>(s, dz, in, B, L, cin, cout, ks, zero_pad != 0, dw, nullptr, part)
-                    : act_wgrad<F, false, false>(s, dz, in, B, L, cin, cout, ks, zero_pad != 0, dw, nullptr, part);
-    });
+    const ActIn in{(const unsigned*)codes, scales, gamma, beta, (const unsigned*)codes_r, scales_r, gamma_r, beta_r,
+                   format == CAMAL_ACT_E4M3, relu != 0, zero_pad != 0};
+    return act_wgrad((hipStream_t)stream, dz, in, B, L, cin, cout, ks, dw, nullptr, (float*)workspace);
 }
 
 }  // extern "C"

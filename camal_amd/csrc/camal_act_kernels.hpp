@@ -284,62 +284,210 @@ __global__ __launch_bounds__(256) void act_bwd_apply_kernel(const float* __restr
     }
 }
 
-// ---- weight gradient from the checkpoint ---------------------------------------------------------------------------------
+// ---- weight gradient from the checkpoint, on MFMA ------------------------------------------------------------------------
 //   dw[co][ci][j] = sum_{b,t} dz[b][t][co] a[b][clamp(t + j - ks/2)][ci],  a = bf16(relu(gamma x + beta) [+ skip])
-// a holds 8 significant bits: the code behind it has 7 (int8) or 4 (e4m3).
-// Partial sums of each split go to part[split][j][co][ci]; wgrad_reduce_kernel adds them in a fixed order.
+// GEMM view: M = co, N = ci, K = time, for every tap j.  v_mfma_f32_32x32x16_bf16 takes 16 timesteps per instruction: lane
+// (i = l & 31, h = l >> 5) feeds 8 consecutive times of channel co_i (A) and ci_i (B).
+//   a holds 8 significant bits (the code behind it has 7 or 4), so it is a bf16 operand without loss.  dz is cut into three
+//   bf16 pieces, each the leading 8 bits of what is left: they add up to it exactly, so the three products, summed in the
+//   instruction's fp32, are an fp32 product sum at a third of the bf16 rate, 5 times the rate of fp32 MFMA.
+// One wave = 32 co x CIW * 32 ci x NTAP taps.  The K index is free as long as A and B agree: half h of the wave takes
+// times 32 h .. 32 h + 31 of a 64-step unit, 8 per instruction, so that a lane walks its channel's times in order:
+//   A: dz straight from global memory into registers (a wave owns its co tile: nobody else needs these values), loaded a
+//      whole unit ahead; rows past the window's end are out of the buffer's range and come back as zeros;
+//   B: the unit's input decoded once per workgroup into LDS as [channel][time], so that a lane reads 8 times with one
+//      ds_read_b128; the pitch of 72 times is an odd number of 16-byte slots (no bank conflicts).  A tap is a shift by j
+//      times: even shifts are other registers of the same 16-time window, odd ones one v_alignbit per register.
+// The splits' partial sums go to part[split][j][co][ci]; wgrad_reduce_kernel adds them in a fixed order.
 struct ActIn {  // the layer's input as checkpoint(s)
     const unsigned* codes; const unsigned char* scales; const float *gamma, *beta;
     const unsigned* codes_r; const unsigned char* scales_r; const float *gamma_r, *beta_r;
+    int e4m3, relu, zero_pad;
 };
 
-// 4 channels (c .. c + 3) of row r of the layer's input, as it takes part in the product
-template <typename F, bool RELU, bool RES>
-__device__ __forceinline__ void act_input(const ActIn& in, size_t r, int cin, int c, float (&a)[4]) {
-    const size_t i = r * (size_t)(cin / 4) + c / 4;
-    float x[4], g[4], b[4];
-    act_load<F>(in.codes, in.scales, i, x);
-    load4(in.gamma + c, g); load4(in.beta + c, b);
+#define ACT_UNIT 64        // timesteps of a unit
+#define ACT_PITCH 72       // times per channel in LDS: a unit and up to 8 more for the taps
+#define ACT_TAPS 8         // taps a wave takes at most
+
+__device__ __forceinline__ void act_decode(const ActIn& in, unsigned w, unsigned e, float (&x)[4]) {
+    if (in.e4m3) ActE4M3::unpack(w, x); else ActI8::unpack(w, x);
+    const float s = act_scale(e);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) { a[k] = fmaf(x[k], g[k], b[k]); if (RELU) a[k] = act_relu(a[k]); }
-    if constexpr (RES) {
-        act_load<F>(in.codes_r, in.scales_r, i, x);
-        load4(in.gamma_r + c, g); load4(in.beta_r + c, b);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) a[k] += fmaf(x[k], g[k], b[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) a[k] = (float)(__bf16)a[k];
+    for (int k = 0; k < 4; ++k) x[k] *= s;
 }
 
-#define ACT_WG_TT 32
-template <typename F, bool RELU, bool RES>
-__global__ __launch_bounds__(256) void act_wgrad_simple_kernel(const float* __restrict__ dz, ActIn in, float* __restrict__ part,
-                                                               int B, int L, int cin, int cout, int ks, int tiles_per_split,
-                                                               bool zero_pad) {
-    __shared__ float s_dz[ACT_WG_TT][32], s_a[ACT_WG_TT][32];
-    const int ci0 = (blockIdx.y % (cin / 32)) * 32, co0 = (blockIdx.y / (cin / 32)) * 32, j = blockIdx.z;
-    const int tpw = (L + ACT_WG_TT - 1) / ACT_WG_TT, total = B * tpw;
-    const int lo = min(total, (int)blockIdx.x * tiles_per_split), hi = min(total, lo + tiles_per_split);
-    const int q = (threadIdx.x & 7) * 4, row = threadIdx.x >> 3;  // 4 columns, one of 32 rows
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};  // dw[co0 + row][ci0 + q ..]
-    for (int tile = lo; tile < hi; ++tile) {
-        const int b = tile / tpw, t = (tile - b * tpw) * ACT_WG_TT + row, p = t + j - (ks >> 1);
-        const int pc = p < 0 ? 0 : (p > L - 1 ? L - 1 : p);
-        float d[4] = {0.f, 0.f, 0.f, 0.f}, a[4] = {0.f, 0.f, 0.f, 0.f};
-        if (t < L) {
-            load4(dz + ((size_t)b * L + t) * cout + co0 + q, d);
-            if (!(zero_pad && p != pc)) act_input<F, RELU, RES>(in, (size_t)b * L + pc, cin, ci0 + q, a);
-        }
-        __syncthreads();
-        store4(&s_dz[row][q], d[0], d[1], d[2], d[3]);
-        store4(&s_a[row][q], a[0], a[1], a[2], a[3]);
-        __syncthreads();
-        for (int k = 0; k < ACT_WG_TT; ++k)
+// waves that share a co tile, each on a unit of its own (narrow layers have fewer co tiles than the workgroup has waves)
+template <int COUT> struct ActWK { static constexpr int V = COUT >= 128 ? 1 : 128 / COUT; };
+
+template <int COUT, int CIW, int NTAP>
+__device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float* __restrict__ dz, const ActIn& in,
+                                               float* __restrict__ part, int B, int L, int cin, int ks, int units_per_split,
+                                               int j0) {
+    constexpr int WK = ActWK<COUT>::V, Q = 8 * CIW, TG = ACT_PITCH / 4, REST = TG * WK, PER = (REST * Q + 255) / 256;
+    constexpr int BUF = WK * 32 * CIW * ACT_PITCH;  // halfwords of one LDS buffer
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 31, h = lane >> 5, wk = wave % WK, cot = blockIdx.z * (4 / WK) + wave / WK;
+    const int ci0 = blockIdx.y % (cin / (32 * CIW)) * 32 * CIW;
+    const int tpw = (L + ACT_UNIT - 1) / ACT_UNIT, total = B * tpw;
+    const int lo = min(total, (int)blockIdx.x * units_per_split), hi = min(total, lo + units_per_split);
+
+    f32x16 acc[NTAP][CIW];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[c] = fmaf(s_dz[k][row], s_a[k][q + c], acc[c]);
+    for (int j = 0; j < NTAP; ++j)
+#pragma unroll
+        for (int w = 0; w < CIW; ++w)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[j][w][k] = 0.f;
+
+    // ---- the input tile: 4 channels x 4 times per item ----
+    const int cq = threadIdx.x % Q, rest0 = threadIdx.x / Q;
+    float g[4], b[4], gr[4] = {0.f, 0.f, 0.f, 0.f}, br[4] = {0.f, 0.f, 0.f, 0.f};
+    load4(in.gamma + ci0 + 4 * cq, g); load4(in.beta + ci0 + 4 * cq, b);
+    if (in.codes_r) { load4(in.gamma_r + ci0 + 4 * cq, gr); load4(in.beta_r + ci0 + 4 * cq, br); }
+    unsigned cw[PER][4], cs[PER][4], rw[PER][4], rs[PER][4];
+    auto row_of = [&](int u0, int p, int r, bool& inside) {  // the item's r-th row of the input, edges clamped
+        const int rest = min(rest0 + p * (256 / Q), REST - 1), u = min(u0 + rest / TG, hi - 1);
+        const int bb = u / tpw, t = (u - bb * tpw) * ACT_UNIT + j0 - (ks >> 1) + (rest % TG) * 4 + r;
+        const int tc = t < 0 ? 0 : (t > L - 1 ? L - 1 : t);
+        inside = t == tc;
+        return (size_t)bb * L + tc;
+    };
+    auto fetch = [&](int u0) {
+#pragma unroll
+        for (int p = 0; p < PER; ++p)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                bool inside;
+                const size_t row = row_of(u0, p, r, inside);
+                const size_t ic = row * (cin / 4) + ci0 / 4 + cq, is = row * (cin / 32) + ci0 / 32 + cq / 8;
+                cw[p][r] = in.codes[ic];
+                cs[p][r] = in.scales[is];
+                if (in.codes_r) { rw[p][r] = in.codes_r[ic]; rs[p][r] = in.scales_r[is]; }
+            }
+    };
+    auto stash = [&](int u0, unsigned short* buf) {
+#pragma unroll
+        for (int p = 0; p < PER; ++p) {
+            float a[4][4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float x[4];
+                act_decode(in, cw[p][r], cs[p][r], x);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { a[r][k] = fmaf(x[k], g[k], b[k]); if (in.relu) a[r][k] = act_relu(a[r][k]); }
+                if (in.codes_r) {
+                    act_decode(in, rw[p][r], rs[p][r], x);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) a[r][k] += fmaf(x[k], gr[k], br[k]);
+                }
+                if (in.zero_pad) {
+                    bool inside;
+                    (void)row_of(u0, p, r, inside);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) a[r][k] = inside ? a[r][k] : 0.f;
+                }
+            }
+            const int rest = rest0 + p * (256 / Q);
+            if (rest < REST) {
+                unsigned short* o = buf + ((rest / TG) * 32 * CIW + 4 * cq) * ACT_PITCH + (rest % TG) * 4;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    *reinterpret_cast<uint2*>(o + k * ACT_PITCH) = make_uint2(pk_bf16(a[0][k], a[1][k]), pk_bf16(a[2][k], a[3][k]));
+            }
+        }
+    };
+
+    // ---- dz of a unit: 4 steps x 8 times of this lane's channel ----
+    unsigned d[4][8];
+    const int voff = ((32 * h) * COUT + 32 * cot + i) * 4;
+    auto load_dz = [&](int u, int s) {
+        const int uc = min(u, hi - 1), bb = uc / tpw, t0 = (uc - bb * tpw) * ACT_UNIT;
+        const int rows = u < hi ? min(ACT_UNIT, L - t0) : 0;
+        __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(dz + ((size_t)bb * L + t0) * COUT), 0, rows * COUT * 4, 0x00027000);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[s][e] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, voff + (8 * s + e) * COUT * 4, 0, 0);
+    };
+
+    if (lo < hi) {
+        fetch(lo);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) load_dz(lo + wk, s);
+        stash(lo, lds);
     }
-    store4(part + (((size_t)blockIdx.x * ks + j) * cout + co0 + row) * cin + ci0 + q, acc[0], acc[1], acc[2], acc[3]);
+    int cur = 0;
+    for (int u0 = lo; u0 < hi; u0 += WK, cur ^= 1) {
+        __syncthreads();
+        const bool more = u0 + WK < hi;
+        if (more) fetch(u0 + WK);
+        const unsigned short* a = lds + cur * BUF + (wk * 32 * CIW + i) * ACT_PITCH + 32 * h;
+        u32x4 x0[CIW], x1[CIW];
+#pragma unroll
+        for (int w = 0; w < CIW; ++w) x0[w] = *reinterpret_cast<const u32x4*>(a + w * 32 * ACT_PITCH);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int w = 0; w < CIW; ++w) x1[w] = *reinterpret_cast<const u32x4*>(a + w * 32 * ACT_PITCH + 8 * (s + 1));
+            u32x4 pc[3];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                unsigned q[2][3];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float v = __builtin_bit_cast(float, d[s][2 * e + k]);
+                    q[k][0] = d[s][2 * e + k];
+                    const float r1 = v - __builtin_bit_cast(float, q[k][0] & 0xFFFF0000u);
+                    q[k][1] = __builtin_bit_cast(unsigned, r1);
+                    q[k][2] = __builtin_bit_cast(unsigned, r1 - __builtin_bit_cast(float, q[k][1] & 0xFFFF0000u));
+                }
+#pragma unroll
+                for (int p = 0; p < 3; ++p) pc[p][e] = __builtin_amdgcn_perm(q[1][p], q[0][p], 0x07060302u);
+            }
+            load_dz(u0 + WK + wk, s);  // this step's registers are free: the same step of the next unit
+            u32x4 bt[NTAP][CIW];
+#pragma unroll
+            for (int w = 0; w < CIW; ++w) {
+                const unsigned x[8] = {x0[w][0], x0[w][1], x0[w][2], x0[w][3], x1[w][0], x1[w][1], x1[w][2], x1[w][3]};
+#pragma unroll
+                for (int j = 0; j < NTAP; ++j)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        bt[j][w][k] = j & 1 ? __builtin_amdgcn_alignbit(x[j / 2 + k + 1], x[j / 2 + k], 16) : x[j / 2 + k];
+                x0[w] = x1[w];
+            }
+#pragma unroll
+            for (int p = 2; p >= 0; --p)
+#pragma unroll
+                for (int j = 0; j < NTAP; ++j)
+#pragma unroll
+                    for (int w = 0; w < CIW; ++w)
+                        acc[j][w] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, pc[p]),
+                                                                            __builtin_bit_cast(bf16x8, bt[j][w]), acc[j][w], 0, 0, 0);
+        }
+        if (more) stash(u0 + WK, lds + (cur ^ 1) * BUF);
+    }
+    // acc[j][w][reg]: column ci = ci0 + 32 w + i, row co = 32 cot + (reg & 3) + 8 (reg >> 2) + 4 h
+#pragma unroll
+    for (int j = 0; j < NTAP; ++j)
+#pragma unroll
+        for (int w = 0; w < CIW; ++w) {
+            float* po = part + ((((size_t)blockIdx.x * WK + wk) * ks + (j0 + j)) * COUT + 32 * cot) * cin + ci0 + 32 * w + i;
+#pragma unroll
+            for (int reg = 0; reg < 16; ++reg) po[(size_t)((reg & 3) + 8 * (reg >> 2) + 4 * h) * cin] = acc[j][w][reg];
+        }
+}
+
+// grid = (splits, tap groups x ci tiles, co groups of 128); the first n_hi tap groups take NHI taps, the others NHI - 1
+template <int COUT, int CIW, int NHI>
+__global__ __launch_bounds__(256, 2) void act_wgrad_kernel(const float* __restrict__ dz, ActIn in, float* __restrict__ part, int B,
+                                                           int L, int cin, int ks, int units_per_split, int n_hi) {
+    __shared__ __align__(16) unsigned short lds[2 * ActWK<COUT>::V * 32 * CIW * ACT_PITCH];
+    const int y = blockIdx.y / (cin / (32 * CIW));
+    if (y < n_hi) {
+        act_wgrad_body<COUT, CIW, NHI>(lds, dz, in, part, B, L, cin, ks, units_per_split, y * NHI);
+    } else {
+        if constexpr (NHI > 1)
+            act_wgrad_body<COUT, CIW, NHI - 1>(lds, dz, in, part, B, L, cin, ks, units_per_split, n_hi * NHI + (y - n_hi) * (NHI - 1));
+    }
 }
 
 }  // namespace camal

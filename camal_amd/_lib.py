@@ -13,7 +13,7 @@ LIB_PATH = os.environ.get("CAMAL_HIP_LIB") or os.path.join(_HERE, "libcamal_hip.
 
 ARCH_CAMAL, ARCH_RESNET = 0, 1
 FP32, BF16 = 0, 1
-ACT_INT8, ACT_E4M3 = 0, 1
+ACT_NONE, ACT_INT8, ACT_E4M3 = -1, 0, 1
 PROF_CLASSES = ("stem", "conv", "conv_cam_head", "post", "other")
 
 
@@ -61,6 +61,8 @@ SIGNATURES = {
     "camal_trainer_create_widths": (_i, [_i, _i, _i, _i, _i, _i, C.POINTER(_vp)]),
     "camal_trainer_param_count_widths": (_sz, [_i, _i, _i]),
     "camal_trainer_running_count_widths": (_sz, [_i]),
+    "camal_trainer_create_act": (_i, [_i, _i, _i, _i, _i, _i, _i, C.POINTER(_vp)]),
+    "camal_trainer_workspace_bytes": (_sz, [_vp]),
     "camal_trainer_destroy": (_i, [_vp]),
     "camal_trainer_set_grad_scale": (_i, [_vp, C.c_float]),
     "camal_train_fwd_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, C.c_float, _vp, _vp, _vp, _vp, _vp]),

@@ -196,6 +196,7 @@ class CamAL(object):
         training_kwargs.setdefault("patience_rlr", 3)
         training_kwargs.setdefault("n_warmup_epochs", 1)
         training_kwargs.setdefault("all_gpu", False)
+        training_kwargs.setdefault("act_checkpoint", None)  # "int8" | "e4m3": activations kept in 8 bits (TrainEngine)
 
         X_train, y_train = train_dataset[0], train_dataset[1]
         X_valid, y_valid = valid_dataset[0], valid_dataset[1]
@@ -229,7 +230,8 @@ class CamAL(object):
                 learning_rate=training_kwargs["lr"], weight_decay=training_kwargs["weight_decay"],
                 patience_es=training_kwargs["patience_es"], patience_rlr=training_kwargs["patience_rlr"],
                 n_warmup_epochs=training_kwargs["n_warmup_epochs"], device=device,
-                all_gpu=training_kwargs["all_gpu"] and not over_devices, data_parallel=not spread and not over_devices)
+                all_gpu=training_kwargs["all_gpu"] and not over_devices, data_parallel=not spread and not over_devices,
+                act_checkpoint=training_kwargs["act_checkpoint"])
             clf_trainer.train(training_kwargs["epochs"])
             clf_trainer.restore_best_weights()
             loss_eval, _ = clf_trainer.evaluate(test_loader)

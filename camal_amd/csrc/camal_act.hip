@@ -1,9 +1,16 @@
-// camal_act_impl.hpp — host side of the 8-bit activation checkpoints (included by camal_hip.hip): argument checks, launch
-// shapes and the camal_act_* entry points.
-#pragma once
-#include <climits>
-
+// camal_act.hip — host side of the 8-bit activation checkpoints: argument checks, launch shapes and the camal_act_* entry
+// points.  A translation unit of its own, so that it compiles beside camal_hip.hip.
+#include "camal_act.hpp"
 #include "camal_act_kernels.hpp"
+
+#include <algorithm>
+#include <climits>
+#include <initializer_list>
+#include <type_traits>
+
+#include "../../include/camal_hip.h"
+
+using namespace camal;
 
 namespace {
 
@@ -11,13 +18,13 @@ inline bool act_channels_ok(int c) { return c == 32 || c == 64 || c == 128 || c 
 inline bool act_aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 inline bool act_format_ok(int f) { return f == CAMAL_ACT_INT8 || f == CAMAL_ACT_E4M3; }
 
-// Calls f(format type); every entry point checks the format first
+// Run-time choices as template arguments: f(constant ...)
 template <typename Fn>
-int act_dispatch(int format, Fn&& f) {
-    return format == CAMAL_ACT_INT8 ? f(ActI8()) : f(ActE4M3());
-}
+int with_format(int format, Fn&& f) { return format == CAMAL_ACT_INT8 ? f(ActI8()) : f(ActE4M3()); }
 template <typename Fn>
-int act_dispatch_c(int c, Fn&& f) {
+int with_flag(bool b, Fn&& f) { return b ? f(std::true_type()) : f(std::false_type()); }
+template <typename Fn>
+int with_channels(int c, Fn&& f) {
     switch (c) {
         case 32: return f(std::integral_constant<int, 32>());
         case 64: return f(std::integral_constant<int, 64>());
@@ -27,8 +34,8 @@ int act_dispatch_c(int c, Fn&& f) {
     return fail(CAMAL_ERR_ARG, "channels must be 32, 64, 128 or 256");
 }
 
-// What the entry points share: null pointers, alignment of the float rows (16-byte loads) and of the codes (4-byte loads)
-int act_check(std::initializer_list<const void*> floats, std::initializer_list<const void*> codes,
+// What the entry points share: the shape, null pointers, alignment of the float rows (16-byte loads) and of the rest (4-byte)
+int act_check(std::initializer_list<const void*> floats, std::initializer_list<const void*> words,
               std::initializer_list<const void*> bytes, long long rows, int channels, int format) {
     if (rows < 1 || rows > INT_MAX) return fail(CAMAL_ERR_ARG, "the number of rows must be in 1 .. 2^31 - 1");
     if (!act_channels_ok(channels)) return fail(CAMAL_ERR_ARG, "channels must be 32, 64, 128 or 256");
@@ -37,7 +44,7 @@ int act_check(std::initializer_list<const void*> floats, std::initializer_list<c
         if (!p) return fail(CAMAL_ERR_ARG, "null argument");
         if (!act_aligned(p, 16)) return fail(CAMAL_ERR_ARG, "float tensors must be 16-byte aligned");
     }
-    for (const void* p : codes) {
+    for (const void* p : words) {
         if (!p) return fail(CAMAL_ERR_ARG, "null argument");
         if (!act_aligned(p, 4)) return fail(CAMAL_ERR_ARG, "codes must be 4-byte aligned");
     }
@@ -48,44 +55,21 @@ int act_check(std::initializer_list<const void*> floats, std::initializer_list<c
 
 inline int act_blocks(size_t work, size_t per_block, int cap) { return (int)std::min<size_t>((work + per_block - 1) / per_block, (size_t)cap); }
 
-template <typename F, bool RELU, bool RES>
-int act_write(hipStream_t s, const float* z, ActNorm n, const float* zr, ActNorm nr, size_t rows, int channels, float* out,
-              void* codes, unsigned char* scales, void* codes_r, unsigned char* scales_r) {
-    const size_t n4 = rows * (size_t)(channels / 4);
-    hipLaunchKernelGGL((act_write_kernel<F, RELU, RES>), dim3(act_blocks(n4, 256 * ACT_ROWS, 4096)), dim3(256), 0, s, z, n, zr, nr,
-                       out, (unsigned*)codes, scales, (unsigned*)codes_r, scales_r, n4, channels / 4 - 1);
-    HIP_TRY(hipGetLastError());
-    return 0;
-}
-
-template <typename F, bool AFFINE, bool RELU, bool RES>
-int act_read(hipStream_t s, const ActIn& in, size_t rows, int channels, float* out) {
-    const size_t n4 = rows * (size_t)(channels / 4);
-    hipLaunchKernelGGL((act_read_kernel<F, AFFINE, RELU, RES>), dim3(act_blocks(n4, 256, 4096)), dim3(256), 0, s, in.codes,
-                       in.scales, in.gamma, in.beta, in.codes_r, in.scales_r, in.gamma_r, in.beta_r, out, n4, channels / 4 - 1);
-    HIP_TRY(hipGetLastError());
-    return 0;
-}
-
-inline size_t act_bwd_blocks(size_t rows) { return (rows + BN_ROWS_PER_BLOCK - 1) / BN_ROWS_PER_BLOCK; }
-// workspace of the norm backward: partial sums [blocks][channels][2] in 64 bits, then the two rows of means
-inline size_t act_bwd_bytes(size_t rows, int channels) {
-    return act_bwd_blocks(rows) * channels * 2 * sizeof(double) + 2 * (size_t)channels * sizeof(float);
-}
+inline size_t act_bwd_blocks(size_t rows) { return (rows + ACT_BWD_ROWS - 1) / ACT_BWD_ROWS; }
 
 template <typename F, int C, bool RELU, bool BCAST>
-int act_norm_bwd(hipStream_t s, const float* da, const void* codes, const unsigned char* scales, const float* invstd,
-                 const float* gamma, const float* beta, int N, int L, float* dz, float* dgamma, float* dbeta, void* ws) {
+int act_norm_bwd_impl(hipStream_t s, const float* da, ActCodes k, const float* invstd, const float* gamma, const float* beta, int N,
+                      int L, float* dz, float* dgamma, float* dbeta, void* ws) {
     const int nb = (int)act_bwd_blocks(N);
     double* partial = (double*)ws;
     float* means = (float*)(partial + (size_t)nb * C * 2);
     const size_t n4 = (size_t)N * (C / 4);
-    hipLaunchKernelGGL((act_bwd_partial_kernel<F, C, RELU, BCAST>), dim3(nb), dim3(256), 0, s, da, (const unsigned*)codes, scales,
-                       gamma, beta, N, L, partial);
-    hipLaunchKernelGGL(act_bwd_final_kernel<C>, dim3(C / BN_FINAL_CPB), dim3(BN_FINAL_THREADS), 0, s, partial, nb, N, means,
+    hipLaunchKernelGGL((act_bwd_partial_kernel<F, C, RELU, BCAST>), dim3(nb), dim3(256), 0, s, da, k.codes, k.scales, gamma, beta, N,
+                       L, partial);
+    hipLaunchKernelGGL(act_bwd_final_kernel<C>, dim3(C / ACT_FINAL_CPB), dim3(ACT_FINAL_THREADS), 0, s, partial, nb, N, means,
                        dgamma, dbeta);
-    hipLaunchKernelGGL((act_bwd_apply_kernel<F, C, RELU, BCAST>), dim3(act_blocks(n4, 256, 4096)), dim3(256), 0, s, da,
-                       (const unsigned*)codes, scales, invstd, gamma, beta, means, n4, L, dz);
+    hipLaunchKernelGGL((act_bwd_apply_kernel<F, C, RELU, BCAST>), dim3(act_blocks(n4, 256, 4096)), dim3(256), 0, s, da, k.codes,
+                       k.scales, invstd, gamma, beta, means, n4, L, dz);
     HIP_TRY(hipGetLastError());
     return 0;
 }
@@ -93,7 +77,7 @@ int act_norm_bwd(hipStream_t s, const float* da, const void* codes, const unsign
 // How the weight gradient is cut up, fixed by the shapes alone: the sums have the same order on every call.
 // Tap groups of nearly equal size (9 = 5 + 4, 25 = 7 + 6 + 6 + 6); CIW = 32-wide ci tiles per wave: two where few taps leave
 // room for the accumulators, so that the pieces of dz serve more products; splits for two workgroups on each of 256 CUs.
-struct ActPlan { int B, L, ciw, wk, groups, n_hi, nhi, nsplit, units; };
+struct ActPlan { int B, L, ciw, wk, groups, n_hi, nhi, nsplit, units, want; };
 ActPlan act_wgrad_plan(int B, int L, int cin, int cout, int ks) {
     ActPlan p;
     p.B = ks == 1 ? 1 : B;  // one tap knows no window edges
@@ -105,14 +89,71 @@ ActPlan act_wgrad_plan(int B, int L, int cin, int cout, int ks) {
     p.ciw = cin >= 64 && p.nhi <= 4 ? 2 : 1;
     p.wk = cout >= 128 ? 1 : 128 / cout;
     const int total = p.B * ((p.L + ACT_UNIT - 1) / ACT_UNIT), iters = (total + p.wk - 1) / p.wk;
-    const int want = std::min(std::max(1, 512 / (p.groups * (cin / (32 * p.ciw)) * std::max(1, cout / 128))), iters);
-    p.units = (iters + want - 1) / want * p.wk;
-    p.nsplit = (total + p.units - 1) / p.units;
+    p.want = std::min(std::max(1, 512 / (p.groups * (cin / (32 * p.ciw)) * std::max(1, cout / 128))), iters);
+    p.units = (iters + p.want - 1) / p.want * p.wk;
+    p.nsplit = (total + p.units - 1) / p.units;  // at most want, which grows with B and L
     return p;
 }
 
-int act_wgrad(hipStream_t s, const float* dz, const ActIn& in, int B, int L, int cin, int cout, int ks, float* dw,
-              float* bias_grad, float* part) {
+}  // namespace
+
+int camal::act_write(hipStream_t s, const float* z, ActNorm n, bool relu, const float* zr, ActNorm nr, size_t rows, int channels,
+                     int format, float* out, ActCodes k, ActCodes kr) {
+    const size_t n4 = rows * (size_t)(channels / 4);
+    with_format(format, [&](auto f) { return with_flag(relu, [&](auto re) { return with_flag(zr != nullptr, [&](auto res) {
+        hipLaunchKernelGGL((act_write_kernel<decltype(f), decltype(re)::value, decltype(res)::value>),
+                           dim3(act_blocks(n4, 256 * ACT_ROWS, 4096)), dim3(256), 0, s, z, n, zr, nr, out, k.codes, k.scales,
+                           kr.codes, kr.scales, n4, channels / 4 - 1);
+        return 0;
+    }); }); });
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+int camal::act_read(hipStream_t s, const ActIn& in, size_t rows, int channels, float* out) {
+    const size_t n4 = rows * (size_t)(channels / 4);
+    with_format(in.e4m3 ? CAMAL_ACT_E4M3 : CAMAL_ACT_INT8, [&](auto f) {
+        auto launch = [&](auto affine, auto relu, auto res) {
+            hipLaunchKernelGGL((act_read_kernel<decltype(f), decltype(affine)::value, decltype(relu)::value, decltype(res)::value>),
+                               dim3(act_blocks(n4, 256, 4096)), dim3(256), 0, s, in.codes, in.scales, in.gamma, in.beta, in.codes_r,
+                               in.scales_r, in.gamma_r, in.beta_r, out, n4, channels / 4 - 1);
+            return 0;
+        };
+        if (!in.gamma) return launch(std::false_type(), std::false_type(), std::false_type());
+        return with_flag(in.relu != 0, [&](auto relu) {
+            return with_flag(in.codes_r != nullptr, [&](auto res) { return launch(std::true_type(), relu, res); }); });
+    });
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+// partial sums [blocks][channels][2] in 64 bits, then the two rows of means
+size_t camal::act_norm_bwd_bytes(size_t rows, int channels) {
+    return act_bwd_blocks(rows) * channels * 2 * sizeof(double) + 2 * (size_t)channels * sizeof(float);
+}
+
+int camal::act_norm_bwd(hipStream_t s, const float* da, bool pooled, ActCodes k, int format, int B, int L, int channels,
+                        const float* invstd, const float* gamma, const float* beta, bool relu, float* dz, float* dgamma,
+                        float* dbeta, void* ws) {
+    return with_format(format, [&](auto f) { return with_channels(channels, [&](auto c) { return with_flag(relu, [&](auto re) {
+        return with_flag(pooled, [&](auto po) {
+            return act_norm_bwd_impl<decltype(f), decltype(c)::value, decltype(re)::value, decltype(po)::value>(
+                s, da, k, invstd, gamma, beta, B * L, L, dz, dgamma, dbeta, ws);
+        }); }); }); });
+}
+
+size_t camal::act_wgrad_bytes(int B, int L, int cin, int cout, int ks) {
+    const ActPlan p = act_wgrad_plan(B, L, cin, cout, ks);
+    return (size_t)p.nsplit * p.wk * ks * cout * cin * sizeof(float);
+}
+
+size_t camal::act_wgrad_max_bytes(int B, int L, int cin, int cout, int ks) {
+    const ActPlan p = act_wgrad_plan(B, L, cin, cout, ks);
+    return (size_t)p.want * p.wk * ks * cout * cin * sizeof(float);
+}
+
+int camal::act_wgrad(hipStream_t s, const float* dz, const ActIn& in, int B, int L, int cin, int cout, int ks, float* dw,
+                     float* bias_grad, float* part) {
     const ActPlan p = act_wgrad_plan(B, L, cin, cout, ks);
     const dim3 grid(p.nsplit, p.groups * (cin / (32 * p.ciw)), std::max(1, cout / 128));
     auto launch = [&](auto co, auto ciw, auto nt) {
@@ -120,7 +161,7 @@ int act_wgrad(hipStream_t s, const float* dz, const ActIn& in, int B, int L, int
                            in, part, p.B, p.L, cin, ks, p.units, p.n_hi);
         return 0;
     };
-    const int rc = act_dispatch_c(cout, [&](auto co) {
+    const int rc = with_channels(cout, [&](auto co) {
 #define CAMAL_ACT_WG(W, N) if (p.ciw == W && p.nhi == N) return launch(co, std::integral_constant<int, W>(), std::integral_constant<int, N>());
         CAMAL_ACT_WG(1, 1) CAMAL_ACT_WG(1, 3) CAMAL_ACT_WG(1, 5) CAMAL_ACT_WG(1, 6) CAMAL_ACT_WG(1, 7) CAMAL_ACT_WG(1, 8)
         CAMAL_ACT_WG(2, 1) CAMAL_ACT_WG(2, 3)
@@ -129,13 +170,11 @@ int act_wgrad(hipStream_t s, const float* dz, const ActIn& in, int B, int L, int
     });
     if (rc) return rc;
     const int total = cout * cin * ks;
-    hipLaunchKernelGGL(wgrad_reduce_kernel, dim3((total / 4 + 63) / 64), dim3(256), 0, s, part, p.nsplit * p.wk, cout, cin, ks, dw,
+    hipLaunchKernelGGL(act_wgrad_reduce_kernel, dim3((total / 4 + 63) / 64), dim3(256), 0, s, part, p.nsplit * p.wk, cout, cin, ks, dw,
                        bias_grad);
     HIP_TRY(hipGetLastError());
     return 0;
 }
-
-}  // namespace
 
 extern "C" {
 
@@ -146,16 +185,8 @@ int camal_act_write(const float* z, const float* mean, const float* invstd, cons
     if (int r = act_check({z, mean, invstd, gamma, beta, out}, {codes}, {scales}, rows, channels, format)) return r;
     if (zr)
         if (int r = act_check({mean_r, invstd_r, gamma_r, beta_r, zr}, {codes_r}, {scales_r}, rows, channels, format)) return r;
-    const ActNorm n{mean, invstd, gamma, beta}, nr{mean_r, invstd_r, gamma_r, beta_r};
-    hipStream_t s = (hipStream_t)stream;
-    return act_dispatch(format, [&](auto f) {
-        using F = decltype(f);
-        if (zr)
-            return relu ? act_write<F, true, true>(s, z, n, zr, nr, rows, channels, out, codes, scales, codes_r, scales_r)
-                        : act_write<F, false, true>(s, z, n, zr, nr, rows, channels, out, codes, scales, codes_r, scales_r);
-        return relu ? act_write<F, true, false>(s, z, n, zr, nr, rows, channels, out, codes, scales, codes_r, scales_r)
-                    : act_write<F, false, false>(s, z, n, zr, nr, rows, channels, out, codes, scales, codes_r, scales_r);
-    });
+    return act_write((hipStream_t)stream, z, {mean, invstd, gamma, beta}, relu != 0, zr, {mean_r, invstd_r, gamma_r, beta_r},
+                     (size_t)rows, channels, format, out, {(unsigned*)codes, scales}, {(unsigned*)codes_r, scales_r});
 }
 
 int camal_act_read(const void* codes, const unsigned char* scales, int format, long long rows, int channels, const float* gamma,
@@ -168,19 +199,14 @@ int camal_act_read(const void* codes, const unsigned char* scales, int format, l
         if (int r = act_check({gamma, beta}, {}, {}, rows, channels, format)) return r;
     if (codes_r)
         if (int r = act_check({gamma_r, beta_r}, {codes_r}, {scales_r}, rows, channels, format)) return r;
-    const ActIn in{(const unsigned*)codes, scales, gamma, beta, (const unsigned*)codes_r, scales_r, gamma_r, beta_r, 0, 0, 0};
-    hipStream_t s = (hipStream_t)stream;
-    return act_dispatch(format, [&](auto f) {
-        using F = decltype(f);
-        if (!gamma) return act_read<F, false, false, false>(s, in, rows, channels, out);
-        if (codes_r)
-            return relu ? act_read<F, true, true, true>(s, in, rows, channels, out) : act_read<F, true, false, true>(s, in, rows, channels, out);
-        return relu ? act_read<F, true, true, false>(s, in, rows, channels, out) : act_read<F, true, false, false>(s, in, rows, channels, out);
-    });
+    return act_read((hipStream_t)stream,
+                    {(const unsigned*)codes, scales, gamma, beta, (const unsigned*)codes_r, scales_r, gamma_r, beta_r,
+                     format == CAMAL_ACT_E4M3, relu != 0, 0},
+                    (size_t)rows, channels, out);
 }
 
 size_t camal_act_norm_bwd_workspace_bytes(long long rows, int channels) {
-    return rows < 1 || rows > INT_MAX || !act_channels_ok(channels) ? 0 : act_bwd_bytes((size_t)rows, channels);
+    return rows < 1 || rows > INT_MAX || !act_channels_ok(channels) ? 0 : act_norm_bwd_bytes((size_t)rows, channels);
 }
 
 int camal_act_norm_bwd(const float* da, int pooled, const void* codes, const unsigned char* scales, int format, int B, int L,
@@ -189,21 +215,10 @@ int camal_act_norm_bwd(const float* da, int pooled, const void* codes, const uns
     if (B < 1 || L < 1) return fail(CAMAL_ERR_ARG, "B and L must be >= 1");
     const long long rows = (long long)B * L;
     if (int r = act_check({da, invstd, gamma, beta, dz, workspace}, {codes, dgamma, dbeta}, {scales}, rows, channels, format)) return r;
-    if (workspace_bytes < act_bwd_bytes((size_t)rows, channels))
+    if (workspace_bytes < act_norm_bwd_bytes((size_t)rows, channels))
         return fail(CAMAL_ERR_ARG, "workspace smaller than camal_act_norm_bwd_workspace_bytes(B * L, channels)");
-    hipStream_t s = (hipStream_t)stream;
-    return act_dispatch(format, [&](auto f) {
-        using F = decltype(f);
-        return act_dispatch_c(channels, [&](auto c) {
-            constexpr int C = decltype(c)::value;
-            const int N = (int)rows;
-            if (pooled)
-                return relu ? act_norm_bwd<F, C, true, true>(s, da, codes, scales, invstd, gamma, beta, N, L, dz, dgamma, dbeta, workspace)
-                            : act_norm_bwd<F, C, false, true>(s, da, codes, scales, invstd, gamma, beta, N, L, dz, dgamma, dbeta, workspace);
-            return relu ? act_norm_bwd<F, C, true, false>(s, da, codes, scales, invstd, gamma, beta, N, L, dz, dgamma, dbeta, workspace)
-                        : act_norm_bwd<F, C, false, false>(s, da, codes, scales, invstd, gamma, beta, N, L, dz, dgamma, dbeta, workspace);
-        });
-    });
+    return act_norm_bwd((hipStream_t)stream, da, pooled != 0, {(unsigned*)codes, (unsigned char*)scales}, format, B, L, channels, invstd,
+                        gamma, beta, relu != 0, dz, dgamma, dbeta, workspace);
 }
 
 static bool act_wgrad_shape_ok(int B, int L, int cin, int cout, int ks) {
@@ -211,9 +226,7 @@ static bool act_wgrad_shape_ok(int B, int L, int cin, int cout, int ks) {
 }
 
 size_t camal_act_wgrad_workspace_bytes(int B, int L, int cin, int cout, int ks) {
-    if (!act_wgrad_shape_ok(B, L, cin, cout, ks)) return 0;
-    const ActPlan p = act_wgrad_plan(B, L, cin, cout, ks);
-    return (size_t)p.nsplit * p.wk * ks * cout * cin * sizeof(float);
+    return act_wgrad_shape_ok(B, L, cin, cout, ks) ? act_wgrad_bytes(B, L, cin, cout, ks) : 0;
 }
 
 int camal_act_wgrad(const float* dz, const void* codes, const unsigned char* scales, int format, int B, int L, int cin, int cout,
@@ -226,11 +239,12 @@ int camal_act_wgrad(const float* dz, const void* codes, const unsigned char* sca
     if (int r = act_check({dz, gamma, beta, workspace}, {codes, dw}, {scales}, rows, cin, format)) return r;
     if (codes_r)
         if (int r = act_check({gamma_r, beta_r}, {codes_r}, {scales_r}, rows, cin, format)) return r;
-    if (workspace_bytes < camal_act_wgrad_workspace_bytes(B, L, cin, cout, ks))
+    if (workspace_bytes < act_wgrad_bytes(B, L, cin, cout, ks))
         return fail(CAMAL_ERR_ARG, "workspace smaller than camal_act_wgrad_workspace_bytes(B, L, cin, cout, ks)");
-    const ActIn in{(const unsigned*)codes, scales, gamma, beta, (const unsigned*)codes_r, scales_r, gamma_r, beta_r,
-                   format == CAMAL_ACT_E4M3, relu != 0, zero_pad != 0};
-    return act_wgrad((hipStream_t)stream, dz, in, B, L, cin, cout, ks, dw, nullptr, (float*)workspace);
+    return act_wgrad((hipStream_t)stream, dz,
+                     {(const unsigned*)codes, scales, gamma, beta, (const unsigned*)codes_r, scales_r, gamma_r, beta_r,
+                      format == CAMAL_ACT_E4M3, relu != 0, zero_pad != 0},
+                     B, L, cin, cout, ks, dw, nullptr, (float*)workspace);
 }
 
 }  // extern "C"

@@ -13,7 +13,7 @@
 // the forward pass's mask element for element; rounding alone flips the 1 to 2 % of the elements that lie within half a
 // step of the threshold, an error of about 10 % in the gradient's norm.
 #pragma once
-#include "camal_train_kernels.hpp"
+#include "camal_act.hpp"
 
 namespace camal {
 
@@ -95,9 +95,6 @@ __device__ __forceinline__ unsigned act_encode(const float (&x)[4], const float 
 // ---- write: a = relu(bn(z)) [+ bn_r(zr)] in fp32, and the checkpoint(s) --------------------------------------------
 // A lane owns 4 channels for the whole launch (the stride between its rows is a multiple of the row), so the statistics
 // stay in registers; ACT_ROWS of its rows are in flight at once.
-struct ActNorm {
-    const float *mean, *invstd, *gamma, *beta;
-};
 #define ACT_ROWS 4
 
 template <typename F, bool RELU, bool RES>
@@ -194,15 +191,17 @@ __global__ __launch_bounds__(256) void act_read_kernel(const unsigned* __restric
 // ---- backward of norm + ReLU from the checkpoint -----------------------------------------------------------------------
 //   dy = da * [fma(x, gamma, beta) > 0],  s1 = sum dy,  s2 = sum dy x,  dz = gamma invstd (dy - s1/N - x s2/N)
 // The sums come first, so the input is read twice by nature.  BCAST: da[b][t][c] = dpool[b][c] / L.
+#define ACT_BWD_ROWS 64  // rows per workgroup of the first stage
+
 template <typename F, int C, bool RELU, bool BCAST>
 __global__ __launch_bounds__(256) void act_bwd_partial_kernel(const float* __restrict__ da, const unsigned* __restrict__ codes,
                                                               const unsigned char* __restrict__ scales,
                                                               const float* __restrict__ gamma, const float* __restrict__ beta,
                                                               int N, int L, double* __restrict__ partial) {
-    constexpr int Q = C / 4, G = 256 / Q, RPL = BN_ROWS_PER_BLOCK / G;
+    constexpr int Q = C / 4, G = 256 / Q, RPL = ACT_BWD_ROWS / G;
     __shared__ float sh[G][C][2];
     const int q4 = threadIdx.x % Q, c4 = q4 * 4, g = threadIdx.x / Q;
-    const int r0 = blockIdx.x * BN_ROWS_PER_BLOCK;
+    const int r0 = blockIdx.x * ACT_BWD_ROWS;
     float ga[4], be[4];
     load4(gamma + c4, ga); load4(beta + c4, be);
     unsigned w[RPL], e[RPL];
@@ -245,14 +244,47 @@ __global__ __launch_bounds__(256) void act_bwd_partial_kernel(const float* __res
     }
 }
 
+// Second stage: ACT_FINAL_CPB channels per workgroup, each lane a fixed strided subset of the partial sums, combined in a fixed
+// order (xor shuffles inside the wave, LDS across the waves).
+#define ACT_FINAL_CPB 8
+#define ACT_FINAL_THREADS 1024
+template <int C>
+__device__ __forceinline__ bool act_final_reduce(const double* __restrict__ partial, int nblocks, int& c, double& a, double& b) {
+    constexpr int G = ACT_FINAL_THREADS / ACT_FINAL_CPB, NW = ACT_FINAL_THREADS / 64;
+    static_assert(C % ACT_FINAL_CPB == 0 && 64 % ACT_FINAL_CPB == 0, "channels per workgroup");
+    __shared__ double sh[NW][ACT_FINAL_CPB][2];
+    const int cl = threadIdx.x % ACT_FINAL_CPB, g = threadIdx.x / ACT_FINAL_CPB;
+    c = blockIdx.x * ACT_FINAL_CPB + cl;
+    double s = 0.0, ss = 0.0;
+#pragma unroll 4
+    for (int i = g; i < nblocks; i += G) {
+        const double2 t = *reinterpret_cast<const double2*>(partial + ((size_t)i * C + c) * 2);
+        s += t.x;
+        ss += t.y;
+    }
+#pragma unroll
+    for (int m = ACT_FINAL_CPB; m < 64; m <<= 1) {
+        s += __shfl_xor(s, m, 64);
+        ss += __shfl_xor(ss, m, 64);
+    }
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (lane < ACT_FINAL_CPB) { sh[wave][lane][0] = s; sh[wave][lane][1] = ss; }
+    __syncthreads();
+    a = 0.0; b = 0.0;
+    if (threadIdx.x >= ACT_FINAL_CPB) return false;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) { a += sh[k][cl][0]; b += sh[k][cl][1]; }
+    return true;
+}
+
 // means[0][c] = s1 / N, means[1][c] = s2 / N for the apply pass
 template <int C>
-__global__ __launch_bounds__(BN_FINAL_THREADS) void act_bwd_final_kernel(const double* __restrict__ partial, int nblocks, int N,
+__global__ __launch_bounds__(ACT_FINAL_THREADS) void act_bwd_final_kernel(const double* __restrict__ partial, int nblocks, int N,
                                                                          float* __restrict__ means, float* __restrict__ dgamma,
                                                                          float* __restrict__ dbeta) {
     double a, b;
     int c;
-    if (!bn_final_reduce<C>(partial, nblocks, c, a, b)) return;
+    if (!act_final_reduce<C>(partial, nblocks, c, a, b)) return;
     means[c] = (float)(a / N);
     means[C + c] = (float)(b / N);
     dbeta[c] = (float)a;
@@ -298,13 +330,7 @@ __global__ __launch_bounds__(256) void act_bwd_apply_kernel(const float* __restr
 //   B: the unit's input decoded once per workgroup into LDS as [channel][time], so that a lane reads 8 times with one
 //      ds_read_b128; the pitch of 72 times is an odd number of 16-byte slots (no bank conflicts).  A tap is a shift by j
 //      times: even shifts are other registers of the same 16-time window, odd ones one v_alignbit per register.
-// The splits' partial sums go to part[split][j][co][ci]; wgrad_reduce_kernel adds them in a fixed order.
-struct ActIn {  // the layer's input as checkpoint(s)
-    const unsigned* codes; const unsigned char* scales; const float *gamma, *beta;
-    const unsigned* codes_r; const unsigned char* scales_r; const float *gamma_r, *beta_r;
-    int e4m3, relu, zero_pad;
-};
-
+// The splits' partial sums go to part[split][j][co][ci]; act_wgrad_reduce_kernel adds them in a fixed order.
 #define ACT_UNIT 64        // timesteps of a unit
 #define ACT_PITCH 72       // times per channel in LDS: a unit and up to 8 more for the taps
 #define ACT_TAPS 8         // taps a wave takes at most
@@ -488,6 +514,37 @@ __global__ __launch_bounds__(256, 2) void act_wgrad_kernel(const float* __restri
         if constexpr (NHI > 1)
             act_wgrad_body<COUT, CIW, NHI - 1>(lds, dz, in, part, B, L, cin, ks, units_per_split, n_hi * NHI + (y - n_hi) * (NHI - 1));
     }
+}
+
+// grad[co][ci][j] = sum_split part[split][j][co][ci]; bias_grad[0..cout) = 0 unless null.  Four ci per lane and
+// four lanes per quad, each walking every fourth split with independent 16-byte loads, combined in a fixed order:
+// one lane per element walking all splits moved the partials at 1.9 TB/s.
+__global__ __launch_bounds__(256) void act_wgrad_reduce_kernel(const float* __restrict__ part, int nsplit, int cout, int cin,
+                                                           int ks, float* __restrict__ grad, float* __restrict__ bias_grad) {
+    __shared__ float4 red[4][64];
+    const int total = cout * cin * ks;
+    const int q = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const int idx = (blockIdx.x * 64 + q) * 4;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (idx < total) {
+#pragma unroll 8
+        for (int s = g; s < nsplit; s += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(part + (size_t)s * total + idx);
+            a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+        }
+    }
+    red[g][q] = a;
+    __syncthreads();
+    if (g == 0 && idx < total) {
+        const float4 b = red[1][q], c = red[2][q], d = red[3][q];
+        const int ci = idx % cin, co = (idx / cin) % cout, j = idx / (cin * cout);
+        float* o = grad + ((size_t)co * cin + ci) * ks + j;
+        o[0] = (a.x + b.x) + (c.x + d.x);
+        o[ks] = (a.y + b.y) + (c.y + d.y);
+        o[2 * ks] = (a.z + b.z) + (c.z + d.z);
+        o[3 * ks] = (a.w + b.w) + (c.w + d.w);
+    }
+    if (bias_grad && blockIdx.x == 0 && threadIdx.x < cout) bias_grad[threadIdx.x] = 0.f;
 }
 
 }  // namespace camal

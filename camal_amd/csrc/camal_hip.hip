@@ -1,6 +1,7 @@
 // camal_hip.hip — host side of libcamal_hip.so: context, weight re-layout, launch sequences.
 // C ABI declared in include/camal_hip.h.  gfx950 only.
 #include "camal_kernels.hpp"
+#include "camal_act.hpp"
 #include "../../include/camal_hip.h"
 
 #include <algorithm>
@@ -16,20 +17,15 @@
 using namespace camal;
 
 namespace {
-
 thread_local std::string g_err;
+}
 
-int fail(int code, const std::string& msg) {
+int camal::fail(int code, const std::string& msg) {
     g_err = msg;
     return code;
 }
 
-#define HIP_TRY(expr)                                                                         \
-    do {                                                                                      \
-        hipError_t e__ = (expr);                                                              \
-        if (e__ != hipSuccess)                                                                \
-            return fail(CAMAL_ERR_HIP, std::string(#expr) + ": " + hipGetErrorString(e__));   \
-    } while (0)
+namespace {
 
 constexpr int C1 = 64, C2 = 128;  // core.py:37 mid_channels default; CamAL.eval ignores kwargs (:386-390)
 
@@ -1262,5 +1258,4 @@ int camal_get_profile(camal_ctx* c, int* launches, double* ms) {
 
 }  // extern "C"
 
-#include "camal_act_impl.hpp"
 #include "camal_train_impl.hpp"

@@ -3,6 +3,9 @@
 // (reference src/helpers/torch_trainer.py:281-298): forward in train() mode (BatchNorm batch
 // statistics), mean cross-entropy, backward, AdamW.
 #pragma once
+#include <climits>
+
+#include "camal_act.hpp"
 #include "camal_train_kernels.hpp"
 
 namespace {
@@ -67,6 +70,13 @@ struct camal_trainer {
     // activations: z (pre-BN conv outputs) and a (post BN/ReLU, block outputs) per layer slot
     float* z[11] = {nullptr};
     float* act[9] = {nullptr};      // a0,a1,out1, a3,a4,out2, a6,a7,out3
+    // with 8-bit activation checkpoints (act_format >= 0): the slots' normalised values as codes and scales; z and act are
+    // then views of the gradient buffers, which the forward pass does not need (z in gZ, the skip's z in gZr, the
+    // activations in turn in gA and gB), and hold only the layer at hand
+    int act_format = CAMAL_ACT_NONE;
+    ActCodes kept[11];
+    bool ckpt() const { return act_format != CAMAL_ACT_NONE; }
+    size_t bytes = 0;               // device memory of the workspace
     float *mean = nullptr, *invstd = nullptr, *s1 = nullptr, *s2 = nullptr;  // [11][256], [256]
     double* partial = nullptr;
     float* wpack[9] = {nullptr};    // forward packing of conv 1..8 (index = conv idx), [0] unused
@@ -87,6 +97,7 @@ namespace {
 int t_alloc(camal_trainer* t, void** p, size_t bytes) {
     HIP_TRY(hipMalloc(p, bytes));
     t->owned.push_back(*p);
+    t->bytes += bytes;
     return 0;
 }
 
@@ -185,9 +196,13 @@ int t_bn_stats_any(camal_trainer* t, hipStream_t s, const float* z, int N, const
     return dispatch_c(l.cout, [&](auto c) { return t_bn_stats<decltype(c)::value>(t, s, z, N, l, 1e-5f, momentum, running); });
 }
 
+int t_keep(camal_trainer* t, hipStream_t s, const float* params, const TLayer& l, const float* z, const TLayer* lr, const float* zr,
+           float* out, int N);
+
 template <int C, bool RELU, bool HAS_RES>
 int t_bn_apply(camal_trainer* t, hipStream_t s, const float* params, const TLayer& l, const float* z, const TLayer* lr,
                const float* zr, float* out, int N) {
+    if (t->ckpt()) return t_keep(t, s, params, l, z, lr, zr, out, N);
     const size_t n4 = (size_t)N * (C / 4);
     hipLaunchKernelGGL((bn_apply_kernel<C, RELU, HAS_RES>), dim3(gs_blocks(n4)), dim3(256), 0, s, z, t->mean + l.zi * 256,
                        t->invstd + l.zi * 256, params + l.g, params + l.be, zr, lr ? t->mean + lr->zi * 256 : nullptr,
@@ -201,6 +216,9 @@ int t_bn_apply(camal_trainer* t, hipStream_t s, const float* params, const TLaye
 template <int C, bool RELU, bool BCAST>
 int t_bn_bwd(camal_trainer* t, hipStream_t s, const float* params, float* grads, const TLayer& l, const float* da,
              const float* z, float* dz, int N, int L) {
+    if (t->ckpt())
+        return act_norm_bwd(s, da, BCAST, t->kept[l.zi], t->act_format, N / L, L, C, t->invstd + l.zi * 256, params + l.g,
+                            params + l.be, RELU, dz, grads + l.g, grads + l.be, t->partial);
     const int nb = (N + BN_ROWS_PER_BLOCK - 1) / BN_ROWS_PER_BLOCK;
     const float* mean = t->mean + l.zi * 256;
     const float* invstd = t->invstd + l.zi * 256;
@@ -215,10 +233,16 @@ int t_bn_bwd(camal_trainer* t, hipStream_t s, const float* params, float* grads,
     return 0;
 }
 
+ActIn t_kept_input(const camal_trainer* t, const float* params, int li);
+
 // weight gradient of a conv layer with cin >= 64 (MFMA), bias gradient = 0 (the bias is
 // followed by a train-mode BatchNorm, which removes any per-channel constant: its exact
 // gradient is zero; torch's value is rounding noise of sum(dz)).
-int t_wgrad(camal_trainer* t, hipStream_t s, const TLayer& l, const float* dz, const float* ain, float* grads, int B, int L) {
+// `li`: the layer reads what conv layer li reads
+int t_wgrad(camal_trainer* t, hipStream_t s, const TLayer& l, int li, const float* params, const float* dz, float* grads, int B, int L) {
+    if (t->ckpt())
+        return act_wgrad(s, dz, t_kept_input(t, params, li), B, L, l.cin, l.cout, l.ks, grads + l.w, grads + l.b, t->wg_part);
+    const float* ain = t->act[li - 1];
     int wps = 1;  // tiles per split
     const int nsplit = wgrad_splits(t, l, B, L, &wps);
     const size_t need = (size_t)nsplit * l.ks * l.cout * l.cin;
@@ -252,6 +276,32 @@ int t_wgrad(camal_trainer* t, hipStream_t s, const TLayer& l, const float* dz, c
                        l.ks, grads + l.w, grads + l.b);
     HIP_TRY(hipGetLastError());
     return 0;
+}
+
+// ---- the same three with 8-bit activation checkpoints ------------------------------------------
+// the input of conv layer li (li >= 1; the input of block 2's skip convolution is that of layer 3) as checkpoint(s)
+ActIn t_kept_input(const camal_trainer* t, const float* params, int li) {
+    const TLayer& l = t->lay.conv[li - 1];
+    const ActCodes& k = t->kept[l.zi];
+    ActIn in{k.codes, k.scales, params + l.g, params + l.be, nullptr, nullptr, nullptr, nullptr,
+             t->act_format == CAMAL_ACT_E4M3, 1, t->zpad()};
+    if (li == 3 || li == 6) {  // the output of blocks 1, 2: the skip branch is part of it
+        const TLayer& lr = t->lay.res[li / 3 - 1];
+        const ActCodes& kr = t->kept[lr.zi];
+        in.codes_r = kr.codes; in.scales_r = kr.scales; in.gamma_r = params + lr.g; in.beta_r = params + lr.be;
+    }
+    return in;
+}
+
+ActNorm t_norm(const camal_trainer* t, const float* params, const TLayer& l) {
+    return {t->mean + l.zi * 256, t->invstd + l.zi * 256, params + l.g, params + l.be};
+}
+
+// forward: normalise, ReLU, add the skip branch, keep
+int t_keep(camal_trainer* t, hipStream_t s, const float* params, const TLayer& l, const float* z, const TLayer* lr, const float* zr,
+           float* out, int N) {
+    return act_write(s, z, t_norm(t, params, l), true, zr, lr ? t_norm(t, params, *lr) : ActNorm{}, N, l.cout, t->act_format, out,
+                     t->kept[l.zi], lr ? t->kept[lr->zi] : ActCodes{});
 }
 
 int t_stem_wgrad(camal_trainer* t, hipStream_t s, const TLayer& l, const float* dz, const float* x, float* grads, int B, int L) {
@@ -322,7 +372,16 @@ int camal_trainer_create_arch(int device_id, int kernel_size, int max_batch, int
 
 int camal_trainer_create_widths(int device_id, int kernel_size, int max_batch, int max_len, int arch, int mid_channels,
                                 camal_trainer** out) {
+    return camal_trainer_create_act(device_id, kernel_size, max_batch, max_len, arch, mid_channels, CAMAL_ACT_NONE, out);
+}
+
+int camal_trainer_create_act(int device_id, int kernel_size, int max_batch, int max_len, int arch, int mid_channels, int act_format,
+                             camal_trainer** out) {
     if (!out) return fail(CAMAL_ERR_ARG, "null argument");
+    if (act_format != CAMAL_ACT_NONE && act_format != CAMAL_ACT_INT8 && act_format != CAMAL_ACT_E4M3)
+        return fail(CAMAL_ERR_ARG, "act_format must be CAMAL_ACT_NONE, CAMAL_ACT_INT8 or CAMAL_ACT_E4M3");
+    if (act_format != CAMAL_ACT_NONE && (long long)max_batch * max_len > INT_MAX)
+        return fail(CAMAL_ERR_ARG, "max_batch * max_len must be below 2^31");
     if (!mid_supported(mid_channels)) return fail(CAMAL_ERR_ARG, "mid_channels must be 32, 64 or 128");
     const int C2 = 2 * mid_channels;  // this model's widest layer (shadows the default)
     if (arch != CAMAL_ARCH_CAMAL && arch != CAMAL_ARCH_RESNET) return fail(CAMAL_ERR_ARG, "arch must be 0 (CamALResNet) or 1 (ResNet)");
@@ -336,6 +395,7 @@ int camal_trainer_create_widths(int device_id, int kernel_size, int max_batch, i
     camal_trainer* t = new camal_trainer();
     t->device = device_id; t->k = kernel_size; t->maxB = max_batch; t->maxL = max_len; t->arch = arch;
     t->mid = mid_channels;
+    t->act_format = act_format;
     t->lay = make_layout(kernel_size, arch, mid_channels);
     hipDeviceProp_t prop;
     if (hipGetDeviceProperties(&prop, device_id) == hipSuccess && prop.multiProcessorCount > 0) t->num_cu = prop.multiProcessorCount;
@@ -346,22 +406,30 @@ int camal_trainer_create_widths(int device_id, int kernel_size, int max_batch, i
     for (int i = 0; i < 9; ++i) zl[t->lay.conv[i].zi] = &t->lay.conv[i];
     zl[t->lay.res[0].zi] = &t->lay.res[0];
     zl[t->lay.res[1].zi] = &t->lay.res[1];
-    for (int i = 0; i < 11; ++i) A(&t->z[i], N * zl[i]->cout);
-    for (int i = 0; i < 9; ++i) A(&t->act[i], N * t->lay.conv[i].cout);
+    if (t->ckpt()) {
+        for (int i = 0; i < 11; ++i) {
+            A(&t->kept[i].codes, N * zl[i]->cout / 4);
+            if (!r) r = t_alloc(t, (void**)&t->kept[i].scales, N * zl[i]->cout / 32);
+        }
+    } else {
+        for (int i = 0; i < 11; ++i) A(&t->z[i], N * zl[i]->cout);
+        for (int i = 0; i < 9; ++i) A(&t->act[i], N * t->lay.conv[i].cout);
+    }
     A(&t->mean, 11 * 256); A(&t->invstd, 11 * 256); A(&t->s1, 256); A(&t->s2, 256);
-    if (!r) r = t_alloc(t, (void**)&t->partial, ((N + BN_ROWS_PER_BLOCK - 1) / BN_ROWS_PER_BLOCK) * 256 * 2 * sizeof(double));
+    if (!r) r = t_alloc(t, (void**)&t->partial, std::max(((N + BN_ROWS_PER_BLOCK - 1) / BN_ROWS_PER_BLOCK) * 256 * 2 * sizeof(double),
+                                                         t->ckpt() ? act_norm_bwd_bytes(N, C2) : 0));
     size_t wg_max = 0;
     for (int i = 1; i < 9; ++i) {
         const TLayer& l = t->lay.conv[i];
         A(&t->wpack[i], (size_t)l.cout * l.cin * l.ks);
         A(&t->wflip[i], (size_t)l.cout * l.cin * l.ks);
-        wg_max = std::max(wg_max, (size_t)wgrad_want(t, l) * l.ks * l.cout * l.cin);
+        wg_max = std::max(wg_max, t->ckpt() ? act_wgrad_max_bytes(max_batch, max_len, l.cin, l.cout, l.ks) / 4 : (size_t)wgrad_want(t, l) * l.ks * l.cout * l.cin);
     }
     {
         const TLayer& l = t->lay.res[1];
         A(&t->wpack_res2, (size_t)l.cout * l.cin);
         A(&t->wflip_res2, (size_t)l.cout * l.cin);
-        wg_max = std::max(wg_max, (size_t)wgrad_want(t, l) * l.cout * l.cin);
+        wg_max = std::max(wg_max, t->ckpt() ? act_wgrad_max_bytes(max_batch, max_len, l.cin, l.cout, 1) / 4 : (size_t)wgrad_want(t, l) * l.cout * l.cin);
     }
     t->wg_part_floats = wg_max;
     A(&t->wg_part, wg_max);
@@ -373,6 +441,10 @@ int camal_trainer_create_widths(int device_id, int kernel_size, int max_batch, i
     A(&t->logits, (size_t)max_batch * 2); A(&t->dlogits, (size_t)max_batch * 2); A(&t->loss, (size_t)max_batch);
     if (!r) r = t_alloc(t, (void**)&t->correct, (size_t)max_batch * sizeof(int));
     A(&t->zeros, 256);
+    if (t->ckpt()) {
+        for (int i = 0; i < 9; ++i) { t->z[t->lay.conv[i].zi] = t->gZ; t->act[i] = i % 2 ? t->gB : t->gA; }
+        t->z[t->lay.res[0].zi] = t->z[t->lay.res[1].zi] = t->gZr;
+    }
     if (!r && hipMemset(t->zeros, 0, 256 * 4) != hipSuccess) r = fail(CAMAL_ERR_HIP, "hipMemset failed");
     if (r) {
         for (void* p : t->owned) (void)hipFree(p);
@@ -391,6 +463,8 @@ int camal_trainer_destroy(camal_trainer* t) {
     delete t;
     return 0;
 }
+
+size_t camal_trainer_workspace_bytes(const camal_trainer* t) { return t ? t->bytes : 0; }
 
 int camal_trainer_set_grad_scale(camal_trainer* t, float scale) {
     if (!t) return fail(CAMAL_ERR_ARG, "null trainer");
@@ -485,7 +559,7 @@ int train_bwd_impl(camal_trainer* t, const float* params, const float* x, const 
             if (lr.cout == C1) r = t_bn_bwd<C1, false, false>(t, s, params, grads, lr, da, t->z[lr.zi], t->gZr, N, L);
             else r = t_bn_bwd<C2, false, false>(t, s, params, grads, lr, da, t->z[lr.zi], t->gZr, N, L);
             if (r) return r;
-            if (b == 1) { if ((r = t_wgrad(t, s, lr, t->gZr, t->act[2], grads, B, L))) return r; }
+            if (b == 1) { if ((r = t_wgrad(t, s, lr, 3, params, t->gZr, grads, B, L))) return r; }
             else { if ((r = t_stem_wgrad(t, s, lr, t->gZr, x, grads, B, L))) return r; }
         }
         for (int i = 2; i >= 0; --i) {
@@ -500,7 +574,7 @@ int train_bwd_impl(camal_trainer* t, const float* params, const float* x, const 
                 if ((r = t_stem_wgrad(t, s, l, t->gZ, x, grads, B, L))) return r;
                 break;
             }
-            if ((r = t_wgrad(t, s, l, t->gZ, t->act[li - 1], grads, B, L))) return r;
+            if ((r = t_wgrad(t, s, l, li, params, t->gZ, grads, B, L))) return r;
             if ((r = t_dgrad(t, s, l, params, t->wflip[li], t->gZ, dnext, B, L))) return r;
             if (li == 3) {  // block 2 input also feeds the 1x1 skip: d(out1) += W_r^T dzr (accumulated in place)
                 const TLayer& lr = Y.res[1];
@@ -554,11 +628,24 @@ int camal_trainer_peek(camal_trainer* t, int what, int index, int B, int L, floa
     if (what == CAMAL_PEEK_ACT) {
         if (index < 0 || index >= 9) return fail(CAMAL_ERR_ARG, "activation index must be 0..8");
         *channels_out = t->lay.conv[index].cout;
+        if (t->ckpt()) return fail(CAMAL_ERR_STATE, "a trainer with 8-bit activation checkpoints keeps no fp32 activations: CAMAL_PEEK_XHAT");
         src = t->act[index];
         n = (size_t)B * L * *channels_out;
     } else {
         if (index < 0 || index >= 11) return fail(CAMAL_ERR_ARG, "slot index must be 0..10");
         *channels_out = zl[index]->cout;
+        if (what == CAMAL_PEEK_Z && t->ckpt())
+            return fail(CAMAL_ERR_STATE, "a trainer with 8-bit activation checkpoints keeps no fp32 activations: CAMAL_PEEK_XHAT");
+        if (what == CAMAL_PEEK_XHAT) {
+            if (!t->ckpt()) return fail(CAMAL_ERR_STATE, "this trainer keeps fp32 activations: CAMAL_PEEK_Z, CAMAL_PEEK_ACT");
+            n = (size_t)B * L * *channels_out;
+            if (!out_dev) return 0;
+            if (out_floats < n) return fail(CAMAL_ERR_ARG, "output buffer too small");
+            HIP_TRY(hipSetDevice(t->device));
+            const ActCodes& k = t->kept[index];
+            return act_read((hipStream_t)stream, ActIn{k.codes, k.scales, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, t->act_format == CAMAL_ACT_E4M3, 0, 0},
+                            (size_t)B * L, *channels_out, out_dev);
+        }
         if (what == CAMAL_PEEK_Z) { src = t->z[index]; n = (size_t)B * L * *channels_out; }
         else if (what == CAMAL_PEEK_MEAN) { src = t->mean + index * 256; n = *channels_out; }
         else if (what == CAMAL_PEEK_INVSTD) { src = t->invstd + index * 256; n = *channels_out; }

@@ -644,7 +644,7 @@ __global__ __launch_bounds__((COUT * 2 * WgCIW<CIN, COUT>::V)) void wgrad_kernel
     }
 }
 
-// grad[co][ci][j] = sum_split part[split][j][co][ci]; bias_grad[0..cout) = 0 (see t_wgrad; null: not written).  Four ci per lane and
+// grad[co][ci][j] = sum_split part[split][j][co][ci]; bias_grad[0..cout) = 0 (see t_wgrad).  Four ci per lane and
 // four lanes per quad, each walking every fourth split with independent 16-byte loads, combined in a fixed order:
 // one lane per element walking all splits moved the partials at 1.9 TB/s.
 __global__ __launch_bounds__(256) void wgrad_reduce_kernel(const float* __restrict__ part, int nsplit, int cout, int cin,
@@ -672,7 +672,7 @@ __global__ __launch_bounds__(256) void wgrad_reduce_kernel(const float* __restri
         o[2 * ks] = (a.z + b.z) + (c.z + d.z);
         o[3 * ks] = (a.w + b.w) + (c.w + d.w);
     }
-    if (bias_grad && blockIdx.x == 0 && threadIdx.x < cout) bias_grad[threadIdx.x] = 0.f;
+    if (blockIdx.x == 0 && threadIdx.x < cout) bias_grad[threadIdx.x] = 0.f;
 }
 
 // Cin = 1 layers: part[b * nseg + seg][j][co] = sum over the segment's t of dz[b][t][co] * x[b][clamp(t + j - pad)]

@@ -184,8 +184,16 @@ class TrainEngine:
 
     BETAS, EPS, BN_MOMENTUM = (0.9, 0.999), 1e-8, 0.1  # torch defaults (AdamW, BatchNorm1d)
 
-    def __init__(self, model, device, max_batch, length, data_parallel=True):
+    ACT_FORMATS = {None: _lib.ACT_NONE, "int8": _lib.ACT_INT8, "e4m3": _lib.ACT_E4M3}
+
+    def __init__(self, model, device, max_batch, length, data_parallel=True, act_checkpoint=None):
+        """``act_checkpoint``: None = the forward pass is kept in fp32 for the backward pass; "int8" or "e4m3" = in one
+        byte per element (``camal_amd.act_checkpoint``): the same forward pass, loss and ReLU masks, a third of the
+        workspace, and gradients that see the activations as the codes hold them."""
         self.lib = _lib.load()
+        if act_checkpoint not in self.ACT_FORMATS:
+            raise ValueError(f"act_checkpoint must be one of {tuple(self.ACT_FORMATS)}, not {act_checkpoint!r}")
+        self.act_checkpoint = act_checkpoint
         # False: this rank trains the member alone (members spread over ranks, CamAL.train)
         self.data_parallel = bool(data_parallel)
         d = torch.device(device)
@@ -204,8 +212,8 @@ class TrainEngine:
         assert self.n == sum(model._params[k].size for k in self.keys)
         self.n_running = int(self.lib.camal_trainer_running_count_widths(self.mid))
         h = C.c_void_p()
-        _lib.check(self.lib.camal_trainer_create_widths(self.device.index, self.k, int(max_batch), int(length), arch_id,
-                                                        self.mid, C.byref(h)))
+        _lib.check(self.lib.camal_trainer_create_act(self.device.index, self.k, int(max_batch), int(length), arch_id,
+                                                     self.mid, self.ACT_FORMATS[act_checkpoint], C.byref(h)))
         self._h = h
         self.max_batch, self.length = int(max_batch), int(length)
         with torch.cuda.device(self.device):
@@ -219,6 +227,11 @@ class TrainEngine:
         self.step_count = 0
         self._grad_scale = 1.0
         self.load_from_model(model)
+
+    @property
+    def workspace_bytes(self):
+        """Device memory of the training workspace (activations kept, gradients in flight, packed weights)."""
+        return int(self.lib.camal_trainer_workspace_bytes(self._h))
 
     def close(self):
         if getattr(self, "_h", None):
@@ -357,12 +370,13 @@ class TrainEngine:
                                                     self.BN_MOMENTUM, None, _lib.ptr(logits), None, None, self._stream()))
         return logits
 
-    PEEK = {"z": 0, "act": 1, "mean": 2, "invstd": 3}
+    PEEK = {"z": 0, "act": 1, "mean": 2, "invstd": 3, "xhat": 4}
 
     def peek(self, what, index, B, L):
         """A copy of what the last forward pass (B windows of L steps) left in the workspace (camal_trainer_peek):
         ``what`` = "z" (pre-BatchNorm conv output of slot ``index`` -> [B, L, C]), "act" (ConvBlock / block output ->
-        [B, L, C]), "mean" / "invstd" (batch statistics -> [C]).  For layer-level parity tests (the reference's
+        [B, L, C]), "mean" / "invstd" (batch statistics -> [C]); with ``act_checkpoint`` "xhat" (normalised values of
+        slot ``index`` as the checkpoint holds them -> [B, L, C]) in place of "z" and "act".  For layer-level parity tests (the reference's
         counterpart is a forward hook on the module)."""
         import ctypes as C
         ch = C.c_int()
@@ -479,7 +493,7 @@ class BasedClassifTrainer(object):
                  criterion=None, patience_es=None, patience_rlr=None, device="cuda", all_gpu=False,
                  valid_criterion=None, n_warmup_epochs=0, f_metrics=Classifmetrics(), verbose=False,
                  plotloss=False, save_fig=False, path_fig=None, save_checkpoint=False, path_checkpoint=None,
-                 data_parallel=True):
+                 data_parallel=True, act_checkpoint=None):
         # criterion (torch_trainer.py:20,52): None or the default nn.CrossEntropyLoss() -> loss and its gradient in the
         # library; anything else is evaluated by torch on the [b, 2] logits of every batch, and the library runs the
         # backward pass from its gradient (camal_train_bwd_dlogits)
@@ -495,8 +509,9 @@ class BasedClassifTrainer(object):
                         path_checkpoint)
         self.model.to(self.device)
         length = train_loader.samples.shape[-1]
-        # data_parallel is not in the reference: see CamAL.member_parallel
-        self.engine = TrainEngine(self.model, self.device, train_loader.batch_size, length, data_parallel=data_parallel)
+        # data_parallel and act_checkpoint are not in the reference: see CamAL.member_parallel, TrainEngine
+        self.engine = TrainEngine(self.model, self.device, train_loader.batch_size, length, data_parallel=data_parallel,
+                                  act_checkpoint=act_checkpoint)
         if all_gpu and not parallel.collectives_on() and torch.cuda.device_count() > 1:
             # the reference's all_gpu=True wraps the model in single-process nn.DataParallel (torch_trainer.py:82-90);
             # here data-parallel training is one process per GPU, which a single process cannot become by itself

@@ -342,17 +342,22 @@ __device__ __forceinline__ void act_decode(const ActIn& in, unsigned w, unsigned
     for (int k = 0; k < 4; ++k) x[k] *= s;
 }
 
-// waves that share a co tile, each on a unit of its own (narrow layers have fewer co tiles than the workgroup has waves)
-template <int COUT> struct ActWK { static constexpr int V = COUT >= 128 ? 1 : 128 / COUT; };
+// Waves of a workgroup (ALL, two per SIMD with what the CU holds), and how many of them share a co tile (WK), each on a unit
+// of its own.  Their accumulators are added in LDS before they leave the workgroup: the partial sums are what bounds the
+// kernel's end (all workgroups write at once) and the reduction behind it.
+template <int COUT> struct ActWaves {
+    static constexpr int ALL = COUT >= 128 ? 8 : 4, CO = COUT >= 128 ? 4 : COUT / 32, WK = ALL / CO;
+};
 
 template <int COUT, int CIW, int NTAP>
 __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float* __restrict__ dz, const ActIn& in,
                                                float* __restrict__ part, int B, int L, int cin, int ks, int units_per_split,
                                                int j0) {
-    constexpr int WK = ActWK<COUT>::V, Q = 8 * CIW, TG = ACT_PITCH / 4, REST = TG * WK, PER = (REST * Q + 255) / 256;
+    constexpr int WK = ActWaves<COUT>::WK, CO = ActWaves<COUT>::CO, NT = 64 * ActWaves<COUT>::ALL;
+    constexpr int Q = 8 * CIW, TG = ACT_PITCH / 4, REST = TG * WK, PER = (REST * Q + NT - 1) / NT;
     constexpr int BUF = WK * 32 * CIW * ACT_PITCH;  // halfwords of one LDS buffer
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int i = lane & 31, h = lane >> 5, wk = wave % WK, cot = blockIdx.z * (4 / WK) + wave / WK;
+    const int i = lane & 31, h = lane >> 5, wk = wave / CO, col = wave % CO, cot = blockIdx.z * CO + col;
     const int ci0 = blockIdx.y % (cin / (32 * CIW)) * 32 * CIW;
     const int tpw = (L + ACT_UNIT - 1) / ACT_UNIT, total = B * tpw;
     const int lo = min(total, (int)blockIdx.x * units_per_split), hi = min(total, lo + units_per_split);
@@ -372,7 +377,7 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
     if (in.codes_r) { load4(in.gamma_r + ci0 + 4 * cq, gr); load4(in.beta_r + ci0 + 4 * cq, br); }
     unsigned cw[PER][4], cs[PER][4], rw[PER][4], rs[PER][4];
     auto row_of = [&](int u0, int p, int r, bool& inside) {  // the item's r-th row of the input, edges clamped
-        const int rest = min(rest0 + p * (256 / Q), REST - 1), u = min(u0 + rest / TG, hi - 1);
+        const int rest = min(rest0 + p * (NT / Q), REST - 1), u = min(u0 + rest / TG, hi - 1);
         const int bb = u / tpw, t = (u - bb * tpw) * ACT_UNIT + j0 - (ks >> 1) + (rest % TG) * 4 + r;
         const int tc = t < 0 ? 0 : (t > L - 1 ? L - 1 : t);
         inside = t == tc;
@@ -413,7 +418,7 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
                     for (int k = 0; k < 4; ++k) a[r][k] = inside ? a[r][k] : 0.f;
                 }
             }
-            const int rest = rest0 + p * (256 / Q);
+            const int rest = rest0 + p * (NT / Q);
             if (rest < REST) {
                 unsigned short* o = buf + ((rest / TG) * 32 * CIW + 4 * cq) * ACT_PITCH + (rest % TG) * 4;
 #pragma unroll
@@ -492,11 +497,25 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
         if (more) stash(u0 + WK, lds + (cur ^ 1) * BUF);
     }
     // acc[j][w][reg]: column ci = ci0 + 32 w + i, row co = 32 cot + (reg & 3) + 8 (reg >> 2) + 4 h
+    float* red = reinterpret_cast<float*>(lds);
 #pragma unroll
     for (int j = 0; j < NTAP; ++j)
 #pragma unroll
         for (int w = 0; w < CIW; ++w) {
-            float* po = part + ((((size_t)blockIdx.x * WK + wk) * ks + (j0 + j)) * COUT + 32 * cot) * cin + ci0 + 32 * w + i;
+            if constexpr (WK > 1) {
+                __syncthreads();
+                if (wk > 0) {
+#pragma unroll
+                    for (int reg = 0; reg < 16; ++reg) red[(((wk - 1) * CO + col) * 16 + reg) * 64 + lane] = acc[j][w][reg];
+                }
+                __syncthreads();
+                if (wk > 0) continue;
+#pragma unroll
+                for (int q = 0; q < WK - 1; ++q)
+#pragma unroll
+                    for (int reg = 0; reg < 16; ++reg) acc[j][w][reg] += red[((q * CO + col) * 16 + reg) * 64 + lane];
+            }
+            float* po = part + (((size_t)blockIdx.x * ks + (j0 + j)) * COUT + 32 * cot) * cin + ci0 + 32 * w + i;
 #pragma unroll
             for (int reg = 0; reg < 16; ++reg) po[(size_t)((reg & 3) + 8 * (reg >> 2) + 4 * h) * cin] = acc[j][w][reg];
         }
@@ -504,9 +523,12 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
 
 // grid = (splits, tap groups x ci tiles, co groups of 128); the first n_hi tap groups take NHI taps, the others NHI - 1
 template <int COUT, int CIW, int NHI>
-__global__ __launch_bounds__(256, 2) void act_wgrad_kernel(const float* __restrict__ dz, ActIn in, float* __restrict__ part, int B,
-                                                           int L, int cin, int ks, int units_per_split, int n_hi) {
-    __shared__ __align__(16) unsigned short lds[2 * ActWK<COUT>::V * 32 * CIW * ACT_PITCH];
+__global__ __launch_bounds__(64 * ActWaves<COUT>::ALL, 2) void act_wgrad_kernel(const float* __restrict__ dz, ActIn in,
+                                                                                float* __restrict__ part, int B, int L, int cin, int ks,
+                                                                                int units_per_split, int n_hi) {
+    using W = ActWaves<COUT>;
+    __shared__ __align__(16) unsigned short lds[2 * W::WK * 32 * CIW * ACT_PITCH];
+    static_assert(sizeof(lds) >= (W::WK - 1) * W::CO * 16 * 64 * sizeof(float), "room for the waves' sums");
     const int y = blockIdx.y / (cin / (32 * CIW));
     if (y < n_hi) {
         act_wgrad_body<COUT, CIW, NHI>(lds, dz, in, part, B, L, cin, ks, units_per_split, y * NHI);
@@ -516,19 +538,21 @@ __global__ __launch_bounds__(256, 2) void act_wgrad_kernel(const float* __restri
     }
 }
 
-// grad[co][ci][j] = sum_split part[split][j][co][ci]; bias_grad[0..cout) = 0 unless null.  Four ci per lane and
-// four lanes per quad, each walking every fourth split with independent 16-byte loads, combined in a fixed order:
-// one lane per element walking all splits moved the partials at 1.9 TB/s.
-__global__ __launch_bounds__(256) void act_wgrad_reduce_kernel(const float* __restrict__ part, int nsplit, int cout, int cin,
-                                                           int ks, float* __restrict__ grad, float* __restrict__ bias_grad) {
-    __shared__ float4 red[4][64];
+// dw[co][ci][j] = sum_split part[split][j][co][ci]; bias_grad[0..cout) = 0 unless null.  Four ci per lane; the splits are dealt
+// to GRP groups of lanes, each with independent 16-byte loads, combined in a fixed order.  A small dw needs many groups to
+// have enough loads in flight.
+template <int GRP>
+__global__ __launch_bounds__(256) void act_wgrad_reduce_kernel(const float* __restrict__ part, int nsplit, int cout, int cin, int ks,
+                                                               float* __restrict__ dw, float* __restrict__ bias_grad) {
+    constexpr int QB = 256 / GRP;
+    __shared__ float4 red[GRP][QB];
     const int total = cout * cin * ks;
-    const int q = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const int idx = (blockIdx.x * 64 + q) * 4;
+    const int q = threadIdx.x % QB, g = threadIdx.x / QB;
+    const int idx = (blockIdx.x * QB + q) * 4;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     if (idx < total) {
 #pragma unroll 8
-        for (int s = g; s < nsplit; s += 4) {
+        for (int s = g; s < nsplit; s += GRP) {
             const float4 v = *reinterpret_cast<const float4*>(part + (size_t)s * total + idx);
             a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
         }
@@ -536,13 +560,17 @@ __global__ __launch_bounds__(256) void act_wgrad_reduce_kernel(const float* __re
     red[g][q] = a;
     __syncthreads();
     if (g == 0 && idx < total) {
-        const float4 b = red[1][q], c = red[2][q], d = red[3][q];
+#pragma unroll
+        for (int k = 1; k < GRP; ++k) {
+            const float4 v = red[k][q];
+            a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+        }
         const int ci = idx % cin, co = (idx / cin) % cout, j = idx / (cin * cout);
-        float* o = grad + ((size_t)co * cin + ci) * ks + j;
-        o[0] = (a.x + b.x) + (c.x + d.x);
-        o[ks] = (a.y + b.y) + (c.y + d.y);
-        o[2 * ks] = (a.z + b.z) + (c.z + d.z);
-        o[3 * ks] = (a.w + b.w) + (c.w + d.w);
+        float* o = dw + ((size_t)co * cin + ci) * ks + j;
+        o[0] = a.x;
+        o[ks] = a.y;
+        o[2 * ks] = a.z;
+        o[3 * ks] = a.w;
     }
     if (bias_grad && blockIdx.x == 0 && threadIdx.x < cout) bias_grad[threadIdx.x] = 0.f;
 }

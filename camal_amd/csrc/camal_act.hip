@@ -76,8 +76,8 @@ int act_norm_bwd_impl(hipStream_t s, const float* da, ActCodes k, const float* i
 
 // How the weight gradient is cut up, fixed by the shapes alone: the sums have the same order on every call.
 // Tap groups of nearly equal size (9 = 5 + 4, 25 = 7 + 6 + 6 + 6); CIW = 32-wide ci tiles per wave: two where few taps leave
-// room for the accumulators, so that the pieces of dz serve more products; splits for 8 waves on each of 256 CUs.
-struct ActPlan { int B, L, ciw, wk, groups, n_hi, nhi, nsplit, units, want; };
+// room for the accumulators, so that the pieces of dz serve more products; splits for one workgroup on each of 256 CUs.
+struct ActPlan { int B, L, ciw, groups, n_hi, nhi, nsplit, units, want; };
 ActPlan act_wgrad_plan(int B, int L, int cin, int cout, int ks) {
     ActPlan p;
     p.B = ks == 1 ? 1 : B;  // one tap knows no window edges
@@ -86,12 +86,12 @@ ActPlan act_wgrad_plan(int B, int L, int cin, int cout, int ks) {
     const int base = ks / p.groups, rem = ks % p.groups;
     p.nhi = rem ? base + 1 : base;
     p.n_hi = rem ? rem : p.groups;
-    p.ciw = cin >= 64 && cout >= 64 && p.nhi <= 4 ? 2 : 1;  // 32 out-channels: four units in LDS leave room for one ci tile
-    p.wk = cout == 32 ? 4 : 2;                               // ActWaves<COUT>::WK
-    const int wgs = cout >= 128 ? 256 : 512;
-    const int total = p.B * ((p.L + ACT_UNIT - 1) / ACT_UNIT), iters = (total + p.wk - 1) / p.wk;
-    p.want = std::min(std::max(1, wgs / (p.groups * (cin / (32 * p.ciw)) * std::max(1, cout / 128))), iters);
-    p.units = (iters + p.want - 1) / p.want * p.wk;
+    p.ciw = cin >= 64 && p.nhi <= 4 ? 2 : 1;
+    const int co = std::min(4, cout / 32), wk = ACT_WAVES / co;  // ActTile<cout>::CO, WK
+    const int tiles = p.groups * (cin / (32 * p.ciw)) * (cout / (32 * co));
+    const int total = p.B * ((p.L + ACT_UNIT - 1) / ACT_UNIT);
+    p.want = std::min(std::max(1, 256 / tiles), (total + wk - 1) / wk);
+    p.units = (total + p.want - 1) / p.want;
     p.nsplit = (total + p.units - 1) / p.units;  // at most want, which grows with B and L
     return p;
 }
@@ -159,7 +159,7 @@ int camal::act_wgrad(hipStream_t s, const float* dz, const ActIn& in, int B, int
     const dim3 grid(p.nsplit, p.groups * (cin / (32 * p.ciw)), std::max(1, cout / 128));
     auto launch = [&](auto co, auto ciw, auto nt) {
         hipLaunchKernelGGL((act_wgrad_kernel<decltype(co)::value, decltype(ciw)::value, decltype(nt)::value>), grid,
-                           dim3(64 * ActWaves<decltype(co)::value>::ALL), 0, s, dz, in, part, p.B, p.L, cin, ks, p.units, p.n_hi);
+                           dim3(64 * ACT_WAVES), 0, s, dz, in, part, p.B, p.L, cin, ks, p.units, p.n_hi);
         return 0;
     };
     const int rc = with_channels(cout, [&](auto co) {
@@ -171,7 +171,7 @@ int camal::act_wgrad(hipStream_t s, const float* dz, const ActIn& in, int B, int
     });
     if (rc) return rc;
     const int quads = cout * cin * ks / 4;
-    if (quads >= 1 << 15)
+    if (quads >= 1 << 15 || p.nsplit <= 16)
         hipLaunchKernelGGL(act_wgrad_reduce_kernel<4>, dim3((quads + 63) / 64), dim3(256), 0, s, part, p.nsplit, cout, cin, ks, dw, bias_grad);
     else
         hipLaunchKernelGGL(act_wgrad_reduce_kernel<16>, dim3((quads + 15) / 16), dim3(256), 0, s, part, p.nsplit, cout, cin, ks, dw, bias_grad);

@@ -323,42 +323,44 @@ __global__ __launch_bounds__(256) void act_bwd_apply_kernel(const float* __restr
 //   a holds 8 significant bits (the code behind it has 7 or 4), so it is a bf16 operand without loss.  dz is cut into three
 //   bf16 pieces, each the leading 8 bits of what is left: they add up to it exactly, so the three products, summed in the
 //   instruction's fp32, are an fp32 product sum at a third of the bf16 rate, 5 times the rate of fp32 MFMA.
-// One wave = 32 co x CIW * 32 ci x NTAP taps.  The K index is free as long as A and B agree: half h of the wave takes
-// times 32 h .. 32 h + 31 of a 64-step unit, 8 per instruction, so that a lane walks its channel's times in order:
-//   A: dz straight from global memory into registers (a wave owns its co tile: nobody else needs these values), loaded a
-//      whole unit ahead; rows past the window's end are out of the buffer's range and come back as zeros;
-//   B: the unit's input decoded once per workgroup into LDS as [channel][time], so that a lane reads 8 times with one
-//      ds_read_b128; the pitch of 72 times is an odd number of 16-byte slots (no bank conflicts).  A tap is a shift by j
-//      times: even shifts are other registers of the same 16-time window, odd ones one v_alignbit per register.
-// The splits' partial sums go to part[split][j][co][ci]; act_wgrad_reduce_kernel adds them in a fixed order.
-#define ACT_UNIT 64        // timesteps of a unit
-#define ACT_PITCH 72       // times per channel in LDS: a unit and up to 8 more for the taps
-#define ACT_TAPS 8         // taps a wave takes at most
+// One wave = 32 co x CIW * 32 ci x NTAP taps on a unit of 64 timesteps.  The 8 waves of a workgroup are CO co tiles x WK units:
+// the CO waves of a unit share its decoded input, and the WK sums of a tile are added in LDS before they leave the workgroup
+// (what the partial sums weigh is what bounds a short call).
+//   A: dz straight from global memory into registers, as the fragment wants it: no other wave needs these values; rows past
+//      the window's end are out of the buffer's range and come back as zeros;
+//   B: the unit's input, decoded into LDS as plain rows [time][32 channels] of bf16, read with the transposing
+//      ds_read_b64_tr_b16 (4 times of a channel per lane): a tap is a row offset, and a row is 64 bytes, so neither side
+//      has bank conflicts.
+// On these SIMDs a vector instruction hides behind a matrix product only up to about three per product (measured: 15.9 ns a
+// product alone, 16.3 with 2, 18.1 with 4, 23.3 with 8 vector instructions to each, two waves), so what counts beside the
+// products is the number of vector instructions: cutting dz takes 44 per 24 products of 8 taps, decoding is shared.
+// Each split's sums go to part[split][j][co][ci]; act_wgrad_reduce_kernel adds them in a fixed order.
+#define ACT_UNIT 64   // timesteps of a unit
+#define ACT_WAVES 8   // waves of a workgroup
+#define ACT_TAPS 8    // taps a wave takes at most
 
-__device__ __forceinline__ void act_decode(const ActIn& in, unsigned w, unsigned e, float (&x)[4]) {
-    if (in.e4m3) ActE4M3::unpack(w, x); else ActI8::unpack(w, x);
-    const float s = act_scale(e);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] *= s;
-}
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
 
-// Waves of a workgroup (ALL, two per SIMD with what the CU holds), and how many of them share a co tile (WK), each on a unit
-// of its own.  Their accumulators are added in LDS before they leave the workgroup: the partial sums are what bounds the
-// kernel's end (all workgroups write at once) and the reduction behind it.
-template <int COUT> struct ActWaves {
-    static constexpr int ALL = COUT >= 128 ? 8 : 4, CO = COUT >= 128 ? 4 : COUT / 32, WK = ALL / CO;
+// How a workgroup is made up, and the passes in which the CO waves of a unit fill its input tile (4 channels per lane)
+template <int COUT, int CIW, int NTAP> struct ActTile {
+    static constexpr int CO = COUT >= 128 ? 4 : COUT / 32, WK = ACT_WAVES / CO;
+    static constexpr int RPW = 8 / CIW, RPP = RPW * CO, ROWS = (ACT_UNIT + NTAP + 6) / 8 * 8, PASS = (ROWS + RPP - 1) / RPP;
+    static constexpr int TILE = CIW * ROWS * 32;  // halfwords
+    // LDS: two tiles per unit, then the waves' sums: ACT_WAVES * (16 - 16 / WK) registers per accumulator, CHUNK of them at once
+    static constexpr int SUMS = ACT_WAVES * (16 - 16 / WK) * 64 * 4, FIT = 128 * 1024 / SUMS;
+    static constexpr int CHUNK = NTAP * CIW < FIT ? NTAP * CIW : FIT;
+    static constexpr int BYTES = 2 * WK * 2 * TILE > CHUNK * SUMS ? 2 * WK * 2 * TILE : CHUNK * SUMS;
 };
 
 template <int COUT, int CIW, int NTAP>
 __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float* __restrict__ dz, const ActIn& in,
                                                float* __restrict__ part, int B, int L, int cin, int ks, int units_per_split,
                                                int j0) {
-    constexpr int WK = ActWaves<COUT>::WK, CO = ActWaves<COUT>::CO, NT = 64 * ActWaves<COUT>::ALL;
-    constexpr int Q = 8 * CIW, TG = ACT_PITCH / 4, REST = TG * WK, PER = (REST * Q + NT - 1) / NT;
-    constexpr int BUF = WK * 32 * CIW * ACT_PITCH;  // halfwords of one LDS buffer
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int i = lane & 31, h = lane >> 5, wk = wave / CO, col = wave % CO, cot = blockIdx.z * CO + col;
-    const int ci0 = blockIdx.y % (cin / (32 * CIW)) * 32 * CIW;
+    using T = ActTile<COUT, CIW, NTAP>;
+    constexpr int CO = T::CO, WK = T::WK;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave / CO, col = wave % CO;
+    const int i = lane & 31, h = lane >> 5, co0 = (blockIdx.z * CO + col) * 32, ci0 = blockIdx.y % (cin / (32 * CIW)) * 32 * CIW;
     const int tpw = (L + ACT_UNIT - 1) / ACT_UNIT, total = B * tpw;
     const int lo = min(total, (int)blockIdx.x * units_per_split), hi = min(total, lo + units_per_split);
 
@@ -370,165 +372,224 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[j][w][k] = 0.f;
 
-    // ---- the input tile: 4 channels x 4 times per item ----
-    const int cq = threadIdx.x % Q, rest0 = threadIdx.x / Q;
+    // ---- the input tile: a lane has 4 channels of every RPP-th row ----
+    const int cq = lane % (8 * CIW), r0 = col * T::RPW + lane / (8 * CIW), lgc = 31 - __builtin_clz(cin);
     float g[4], b[4], gr[4] = {0.f, 0.f, 0.f, 0.f}, br[4] = {0.f, 0.f, 0.f, 0.f};
     load4(in.gamma + ci0 + 4 * cq, g); load4(in.beta + ci0 + 4 * cq, b);
     if (in.codes_r) { load4(in.gamma_r + ci0 + 4 * cq, gr); load4(in.beta_r + ci0 + 4 * cq, br); }
-    unsigned cw[PER][4], cs[PER][4], rw[PER][4], rs[PER][4];
-    auto row_of = [&](int u0, int p, int r, bool& inside) {  // the item's r-th row of the input, edges clamped
-        const int rest = min(rest0 + p * (NT / Q), REST - 1), u = min(u0 + rest / TG, hi - 1);
-        const int bb = u / tpw, t = (u - bb * tpw) * ACT_UNIT + j0 - (ks >> 1) + (rest % TG) * 4 + r;
-        const int tc = t < 0 ? 0 : (t > L - 1 ? L - 1 : t);
-        inside = t == tc;
-        return (size_t)bb * L + tc;
+    const float floor = in.relu ? 0.f : -__builtin_inff();
+    // The tile's codes travel in registers a whole unit ahead.  The tile at (bb, tt): rows relative to its first one, edges
+    // clamped, so that offsets are small.
+    unsigned cw[T::PASS], cs[T::PASS], rw[T::PASS], rs[T::PASS];
+    struct Source { __amdgpu_buffer_rsrc_t codes, scales, codes_r, scales_r; int tb, rb; };
+    auto source = [&](int bb, int tt) {
+        Source o;
+        o.tb = tt * ACT_UNIT + j0 - (ks >> 1);
+        o.rb = max(0, min(o.tb, L - 1));
+        const int rows = min(L - o.rb, 2 * ACT_UNIT);
+        const size_t first = (size_t)bb * L + o.rb;
+        auto rsrc = [&](const void* p, int lg) {
+            return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)p + (first << lg)), 0, rows << lg, 0x00027000);
+        };
+        o.codes = rsrc(in.codes, lgc);
+        o.scales = rsrc(in.scales, lgc - 5);
+        o.codes_r = rsrc(in.codes_r, lgc);  // not read from without a skip branch
+        o.scales_r = rsrc(in.scales_r, lgc - 5);
+        return o;
     };
-    auto fetch = [&](int u0) {
-#pragma unroll
-        for (int p = 0; p < PER; ++p)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                bool inside;
-                const size_t row = row_of(u0, p, r, inside);
-                const size_t ic = row * (cin / 4) + ci0 / 4 + cq, is = row * (cin / 32) + ci0 / 32 + cq / 8;
-                cw[p][r] = in.codes[ic];
-                cs[p][r] = in.scales[is];
-                if (in.codes_r) { rw[p][r] = in.codes_r[ic]; rs[p][r] = in.scales_r[is]; }
-            }
-    };
-    auto stash = [&](int u0, unsigned short* buf) {
-#pragma unroll
-        for (int p = 0; p < PER; ++p) {
-            float a[4][4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float x[4];
-                act_decode(in, cw[p][r], cs[p][r], x);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) { a[r][k] = fmaf(x[k], g[k], b[k]); if (in.relu) a[r][k] = act_relu(a[r][k]); }
-                if (in.codes_r) {
-                    act_decode(in, rw[p][r], rs[p][r], x);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) a[r][k] += fmaf(x[k], gr[k], br[k]);
-                }
-                if (in.zero_pad) {
-                    bool inside;
-                    (void)row_of(u0, p, r, inside);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) a[r][k] = inside ? a[r][k] : 0.f;
-                }
-            }
-            const int rest = rest0 + p * (NT / Q);
-            if (rest < REST) {
-                unsigned short* o = buf + ((rest / TG) * 32 * CIW + 4 * cq) * ACT_PITCH + (rest % TG) * 4;
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    *reinterpret_cast<uint2*>(o + k * ACT_PITCH) = make_uint2(pk_bf16(a[0][k], a[1][k]), pk_bf16(a[2][k], a[3][k]));
-            }
+    auto fetch = [&](const Source& o, int p) {
+        if (col * T::RPW + p * T::RPP >= T::ROWS) return;
+        const int rel = max(-o.rb, min(o.tb - o.rb + r0 + p * T::RPP, L - 1 - o.rb));
+        const int oc = (rel << lgc) + ci0 + 4 * cq, os = (rel << (lgc - 5)) + ci0 / 32 + cq / 8;
+        cw[p] = __builtin_amdgcn_raw_buffer_load_b32(o.codes, oc, 0, 0);
+        cs[p] = __builtin_amdgcn_raw_buffer_load_b8(o.scales, os, 0, 0);
+        if (in.codes_r) {
+            rw[p] = __builtin_amdgcn_raw_buffer_load_b32(o.codes_r, oc, 0, 0);
+            rs[p] = __builtin_amdgcn_raw_buffer_load_b8(o.scales_r, os, 0, 0);
         }
     };
-
-    // ---- dz of a unit: 4 steps x 8 times of this lane's channel ----
-    unsigned d[4][8];
-    const int voff = ((32 * h) * COUT + 32 * cot + i) * 4;
-    auto load_dz = [&](int u, int s) {
-        const int uc = min(u, hi - 1), bb = uc / tpw, t0 = (uc - bb * tpw) * ACT_UNIT;
-        const int rows = u < hi ? min(ACT_UNIT, L - t0) : 0;
-        __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(dz + ((size_t)bb * L + t0) * COUT), 0, rows * COUT * 4, 0x00027000);
+    auto stash = [&](unsigned short* tile, int tb, int p) {
+        if (col * T::RPW + p * T::RPP >= T::ROWS) return;
+        float a[4];
+        if (in.e4m3) ActE4M3::unpack(cw[p], a); else ActI8::unpack(cw[p], a);
+        const float sc = act_scale(cs[p]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d[s][e] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, voff + (8 * s + e) * COUT * 4, 0, 0);
+        for (int k = 0; k < 4; ++k) a[k] = __builtin_elementwise_maximum(fmaf(a[k] * sc, g[k], b[k]), floor);
+        if (in.codes_r) {
+            float x[4];
+            if (in.e4m3) ActE4M3::unpack(rw[p], x); else ActI8::unpack(rw[p], x);
+            const float sr = act_scale(rs[p]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) a[k] += fmaf(x[k] * sr, gr[k], br[k]);
+        }
+        const int row = r0 + p * T::RPP;
+        if (in.zero_pad) {
+            const bool inside = (unsigned)(tb + row) < (unsigned)L;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) a[k] = inside ? a[k] : 0.f;
+        }
+        *reinterpret_cast<uint2*>(tile + ((cq / 8) * T::ROWS + row) * 32 + 4 * (cq % 8)) = make_uint2(pk_bf16(a[0], a[1]), pk_bf16(a[2], a[3]));
     };
 
+    // ---- dz: 8 times of this lane's channel per step, loaded two steps before it is cut, cut a step before it is used ----
+    unsigned d[2][8];
+    u32x4 pc[2][3];
+    const int voff = (8 * h * COUT + co0 + i) * 4;
+    auto load_dz = [&](__amdgpu_buffer_rsrc_t src, int s) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[s & 1][e] = __builtin_amdgcn_raw_buffer_load_b32(src, voff + (16 * s + e) * COUT * 4, 0, 0);
+    };
+    auto cut = [&](int s, int e) {  // times 2 e, 2 e + 1 of step s
+        unsigned q[2][3];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float v = __builtin_bit_cast(float, d[s & 1][2 * e + k]);
+            q[k][0] = d[s & 1][2 * e + k];
+            const float r1 = v - __builtin_bit_cast(float, q[k][0] & 0xFFFF0000u);
+            q[k][1] = __builtin_bit_cast(unsigned, r1);
+            q[k][2] = __builtin_bit_cast(unsigned, r1 - __builtin_bit_cast(float, q[k][1] & 0xFFFF0000u));
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) pc[s & 1][p][e] = __builtin_amdgcn_perm(q[1][p], q[0][p], 0x07060302u);
+    };
+
+    // ---- the B operand: lane's place in a transposing read is rows 8 h + (l % 16) / 4 (+ 4), channels 16 ((l / 16) & 1) +
+    // 4 (l % 4) .. + 3 ----
+    constexpr int TRIOS = NTAP * CIW;
+    const int bp = (8 * h + (lane & 15) / 4) * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    auto operand = [&](const unsigned short* tile, int s, int n) {  // trio n = tap * CIW + ci tile
+        typedef __attribute__((address_space(3))) s16x4 lds4;
+        const unsigned short* q = tile + bp + ((n % CIW) * T::ROWS + 16 * s + n / CIW) * 32;
+        const s16x4 b0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)q);
+        const s16x4 b1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(q + 4 * 32));
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+
+    // The positions of the unit at hand, the next one (whose tile is decoded meanwhile) and the one after it (whose codes are
+    // fetched).  Past the split's end the last unit repeats, and counts for nothing: no rows of dz.
+    auto dz_source = [&](int bb, int tt, bool live) {
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(dz + ((size_t)bb * L + tt * ACT_UNIT) * COUT), 0,
+                                                 live ? min(ACT_UNIT, L - tt * ACT_UNIT) * COUT * 4 : 0, 0x00027000);
+    };
+    int u = min(lo + wk, hi - 1), bb = u / tpw, tt = u - bb * tpw;
+    auto advance = [&]() {
+        const int step = min(WK, hi - 1 - u);
+        u += step;
+        tt += step;
+        while (tt >= tpw) { tt -= tpw; ++bb; }
+    };
+    unsigned short* mine = lds + wk * 2 * T::TILE;  // two tiles: one is read, the other filled
     if (lo < hi) {
-        fetch(lo);
+        Source at = source(bb, tt);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) load_dz(lo + wk, s);
-        stash(lo, lds);
+        for (int p = 0; p < T::PASS; ++p) fetch(at, p);
+        __amdgpu_buffer_rsrc_t dsrc = dz_source(bb, tt, lo + wk < hi);
+        load_dz(dsrc, 0);
+        load_dz(dsrc, 1);
+#pragma unroll
+        for (int p = 0; p < T::PASS; ++p) stash(mine, at.tb, p);
+        advance();
+        at = source(bb, tt);
+#pragma unroll
+        for (int p = 0; p < T::PASS; ++p) fetch(at, p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) cut(0, e);
+        load_dz(dsrc, 2);
+        int cur = 0;
+        for (int u0 = lo; u0 < hi; u0 += WK, cur ^= 1) {
+            unsigned short *now = mine + cur * T::TILE, *next = mine + (cur ^ 1) * T::TILE;
+            const int tb_next = at.tb;
+            const __amdgpu_buffer_rsrc_t dnext = dz_source(bb, tt, u0 + WK + wk < hi);
+            advance();
+            at = source(bb, tt);
+            __syncthreads();
+            bf16x8 bt = operand(now, 0, 0);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                // Between the products of step s: the next step's dz is cut and its registers loaded again, a quarter of the
+                // next tile decoded and its codes fetched again.  In clumps of their own these would leave the matrix pipe
+                // idle (the two waves of a SIMD share it evenly, reach their clumps together and overlap nothing).
+                constexpr int STASH = (T::PASS + 3) / 4, TASKS = 5 + STASH;
+#pragma unroll
+                for (int n = 0; n < TRIOS; ++n) {
+                    bf16x8 bn;
+                    if (n + 1 < TRIOS) bn = operand(now, s, n + 1);
+                    else if (s < 3) bn = operand(now, s + 1, 0);
+#pragma unroll
+                    for (int p = 2; p >= 0; --p)
+                        acc[n / CIW][n % CIW] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, pc[s & 1][p]), bt,
+                                                                                       acc[n / CIW][n % CIW], 0, 0, 0);
+#pragma unroll
+                    for (int t = 0; t < TASKS; ++t) {
+                        if (t * TRIOS / TASKS != n) continue;
+                        if (t < 4) cut(s + 1, t);
+                        else if (t == 4) { if (s == 0) load_dz(dsrc, 3); else load_dz(dnext, s - 1); }
+                        else {
+                            const int p = (t - 5) * 4 + s;
+                            if (p < T::PASS) { stash(next, tb_next, p); fetch(at, p); }
+                        }
+                    }
+                    bt = bn;
+                }
+            }
+            dsrc = dnext;
+        }
     }
-    int cur = 0;
-    for (int u0 = lo; u0 < hi; u0 += WK, cur ^= 1) {
+    // acc[j][w][reg] of lane l: row co = co0 + (reg & 3) + 8 (reg >> 2) + 4 h, column ci = ci0 + 32 w + i.  Of a tile's 16
+    // registers each of its WK waves adds OWN and hands the others out through LDS, as many tiles at once as fit: the
+    // workgroup has the CU to itself.
+    constexpr int OWN = 16 / WK, V = OWN < 4 ? OWN : 4, CHUNK = T::CHUNK;
+    typedef float fv __attribute__((ext_vector_type(V)));
+    fv* red = reinterpret_cast<fv*>(lds);
+    auto slot = [&](int tile, int owner, int from, int k) {  // registers k V .. of what `from` gives `owner`
+        return ((((tile * WK + owner) * (WK - 1) + (from < owner ? from : from - 1)) * CO + col) * (OWN / V) + k) * 64 + lane;
+    };
+#pragma unroll
+    for (int n0 = 0; n0 < TRIOS; n0 += CHUNK) {
         __syncthreads();
-        const bool more = u0 + WK < hi;
-        if (more) fetch(u0 + WK);
-        const unsigned short* a = lds + cur * BUF + (wk * 32 * CIW + i) * ACT_PITCH + 32 * h;
-        u32x4 x0[CIW], x1[CIW];
 #pragma unroll
-        for (int w = 0; w < CIW; ++w) x0[w] = *reinterpret_cast<const u32x4*>(a + w * 32 * ACT_PITCH);
+        for (int n = n0; n < n0 + CHUNK && n < TRIOS; ++n)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
+            for (int owner = 0; owner < WK; ++owner)
+                if (owner != wk)
 #pragma unroll
-            for (int w = 0; w < CIW; ++w) x1[w] = *reinterpret_cast<const u32x4*>(a + w * 32 * ACT_PITCH + 8 * (s + 1));
-            u32x4 pc[3];
+                    for (int k = 0; k < OWN / V; ++k) {
+                        fv v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                unsigned q[2][3];
+                        for (int c = 0; c < V; ++c) v[c] = acc[n / CIW][n % CIW][owner * OWN + k * V + c];
+                        red[slot(n - n0, owner, wk, k)] = v;
+                    }
+        __syncthreads();
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float v = __builtin_bit_cast(float, d[s][2 * e + k]);
-                    q[k][0] = d[s][2 * e + k];
-                    const float r1 = v - __builtin_bit_cast(float, q[k][0] & 0xFFFF0000u);
-                    q[k][1] = __builtin_bit_cast(unsigned, r1);
-                    q[k][2] = __builtin_bit_cast(unsigned, r1 - __builtin_bit_cast(float, q[k][1] & 0xFFFF0000u));
+        for (int owner = 0; owner < WK; ++owner)
+            if (owner == wk)
+#pragma unroll
+                for (int n = n0; n < n0 + CHUNK && n < TRIOS; ++n) {
+                    float* po = part + ((size_t)(blockIdx.x * ks + j0 + n / CIW) * COUT + co0 + 4 * h) * cin + ci0 + 32 * (n % CIW) + i;
+#pragma unroll
+                    for (int k = 0; k < OWN / V; ++k) {
+                        fv v;
+#pragma unroll
+                        for (int c = 0; c < V; ++c) v[c] = acc[n / CIW][n % CIW][owner * OWN + k * V + c];
+#pragma unroll
+                        for (int from = 0; from < WK; ++from)
+                            if (from != owner) v += red[slot(n - n0, owner, from, k)];
+#pragma unroll
+                        for (int c = 0; c < V; ++c) {
+                            const int reg = owner * OWN + k * V + c;
+                            po[(size_t)((reg & 3) + 8 * (reg >> 2)) * cin] = v[c];
+                        }
+                    }
                 }
-#pragma unroll
-                for (int p = 0; p < 3; ++p) pc[p][e] = __builtin_amdgcn_perm(q[1][p], q[0][p], 0x07060302u);
-            }
-            load_dz(u0 + WK + wk, s);  // this step's registers are free: the same step of the next unit
-            u32x4 bt[NTAP][CIW];
-#pragma unroll
-            for (int w = 0; w < CIW; ++w) {
-                const unsigned x[8] = {x0[w][0], x0[w][1], x0[w][2], x0[w][3], x1[w][0], x1[w][1], x1[w][2], x1[w][3]};
-#pragma unroll
-                for (int j = 0; j < NTAP; ++j)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        bt[j][w][k] = j & 1 ? __builtin_amdgcn_alignbit(x[j / 2 + k + 1], x[j / 2 + k], 16) : x[j / 2 + k];
-                x0[w] = x1[w];
-            }
-#pragma unroll
-            for (int p = 2; p >= 0; --p)
-#pragma unroll
-                for (int j = 0; j < NTAP; ++j)
-#pragma unroll
-                    for (int w = 0; w < CIW; ++w)
-                        acc[j][w] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, pc[p]),
-                                                                            __builtin_bit_cast(bf16x8, bt[j][w]), acc[j][w], 0, 0, 0);
-        }
-        if (more) stash(u0 + WK, lds + (cur ^ 1) * BUF);
     }
-    // acc[j][w][reg]: column ci = ci0 + 32 w + i, row co = 32 cot + (reg & 3) + 8 (reg >> 2) + 4 h
-    float* red = reinterpret_cast<float*>(lds);
-#pragma unroll
-    for (int j = 0; j < NTAP; ++j)
-#pragma unroll
-        for (int w = 0; w < CIW; ++w) {
-            if constexpr (WK > 1) {
-                __syncthreads();
-                if (wk > 0) {
-#pragma unroll
-                    for (int reg = 0; reg < 16; ++reg) red[(((wk - 1) * CO + col) * 16 + reg) * 64 + lane] = acc[j][w][reg];
-                }
-                __syncthreads();
-                if (wk > 0) continue;
-#pragma unroll
-                for (int q = 0; q < WK - 1; ++q)
-#pragma unroll
-                    for (int reg = 0; reg < 16; ++reg) acc[j][w][reg] += red[((q * CO + col) * 16 + reg) * 64 + lane];
-            }
-            float* po = part + (((size_t)blockIdx.x * ks + (j0 + j)) * COUT + 32 * cot) * cin + ci0 + 32 * w + i;
-#pragma unroll
-            for (int reg = 0; reg < 16; ++reg) po[(size_t)((reg & 3) + 8 * (reg >> 2) + 4 * h) * cin] = acc[j][w][reg];
-        }
 }
 
-// grid = (splits, tap groups x ci tiles, co groups of 128); the first n_hi tap groups take NHI taps, the others NHI - 1
+// grid = (splits, tap groups x ci tiles, groups of CO co tiles); the first n_hi tap groups take NHI taps, the others NHI - 1
 template <int COUT, int CIW, int NHI>
-__global__ __launch_bounds__(64 * ActWaves<COUT>::ALL, 2) void act_wgrad_kernel(const float* __restrict__ dz, ActIn in,
-                                                                                float* __restrict__ part, int B, int L, int cin, int ks,
-                                                                                int units_per_split, int n_hi) {
-    using W = ActWaves<COUT>;
-    __shared__ __align__(16) unsigned short lds[2 * W::WK * 32 * CIW * ACT_PITCH];
-    static_assert(sizeof(lds) >= (W::WK - 1) * W::CO * 16 * 64 * sizeof(float), "room for the waves' sums");
+__global__ __launch_bounds__(64 * ACT_WAVES, 2) void act_wgrad_kernel(const float* __restrict__ dz, ActIn in, float* __restrict__ part,
+                                                                      int B, int L, int cin, int ks, int units_per_split, int n_hi) {
+    using T = ActTile<COUT, CIW, NHI>;
+    __shared__ __align__(16) unsigned short lds[T::BYTES / 2];
     const int y = blockIdx.y / (cin / (32 * CIW));
     if (y < n_hi) {
         act_wgrad_body<COUT, CIW, NHI>(lds, dz, in, part, B, L, cin, ks, units_per_split, y * NHI);

@@ -13,7 +13,6 @@ current stream of that GPU.
 """
 from __future__ import annotations
 
-import ctypes as C
 from dataclasses import dataclass
 
 import torch
@@ -95,8 +94,28 @@ def _skip(skip, ckpt):
     return codes, scales, _floats(gamma, n, ckpt.device, "skip gamma"), _floats(beta, n, ckpt.device, "skip beta")
 
 
-def _stream(device):
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(device, fn, *args):
+    """``fn(*args, stream)`` on the tensors' GPU and its current stream."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if torch.cuda.current_device() == device.index:
+        code = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            code = fn(*args, stream)
+    if code:
+        _lib.check(code)
+
+
+def _new(z, dtype):
+    """An unwritten checkpoint of z's shape (which the caller has looked over)."""
+    kept = object.__new__(ActivationCheckpoint)
+    object.__setattr__(kept, "codes", torch.empty_like(z, dtype=dtype))
+    object.__setattr__(kept, "scales", z.new_empty((z.shape[0], z.shape[1], z.shape[2] // BLOCK), dtype=torch.uint8))
+    return kept
 
 
 def write(z, mean, invstd, gamma, beta, relu=True, fmt="int8", skip=None):
@@ -116,16 +135,15 @@ def write(z, mean, invstd, gamma, beta, relu=True, fmt="int8", skip=None):
     if skip is not None:
         names = ("skip z", "skip mean", "skip invstd", "skip gamma", "skip beta")
         r = [_floats(t, s, dev, n) for t, s, n in zip(skip, (z.shape, *((ch,),) * 4), names, strict=True)]
-    with torch.cuda.device(dev):
-        out = torch.empty((B, L, ch), dtype=torch.float32, device=dev)
-        kept = [ActivationCheckpoint(torch.empty((B, L, ch), dtype=dtype, device=dev),
-                                     torch.empty((B, L, ch // BLOCK), dtype=torch.uint8, device=dev))
-                for _ in range(1 if skip is None else 2)]
-        second = kept[1] if skip is not None else None
-        _lib.check(_lib.load().camal_act_write(
-            *map(_lib.ptr, a), int(bool(relu)), *map(_lib.ptr, r), B * L, ch, code, _lib.ptr(out), _lib.ptr(kept[0].codes),
-            _lib.ptr(kept[0].scales), _lib.ptr(second and second.codes), _lib.ptr(second and second.scales), _stream(dev)))
-    return (out, *kept)
+    out, kept = torch.empty_like(a[0]), _new(a[0], dtype)
+    if skip is None:
+        _call(dev, _lib.load().camal_act_write, *map(_ptr, a), int(bool(relu)), *r, B * L, ch, code, out.data_ptr(),
+              kept.codes.data_ptr(), kept.scales.data_ptr(), None, None)
+        return out, kept
+    side = _new(a[0], dtype)
+    _call(dev, _lib.load().camal_act_write, *map(_ptr, a), int(bool(relu)), *map(_ptr, r), B * L, ch, code, out.data_ptr(),
+          kept.codes.data_ptr(), kept.scales.data_ptr(), side.codes.data_ptr(), side.scales.data_ptr())
+    return out, kept, side
 
 
 def read(ckpt, gamma=None, beta=None, relu=True, skip=None):
@@ -139,11 +157,9 @@ def read(ckpt, gamma=None, beta=None, relu=True, skip=None):
     if gamma is not None:
         g, b = _floats(gamma, (ch,), dev, "gamma"), _floats(beta, (ch,), dev, "beta")
     r = _skip(skip, ckpt)
-    with torch.cuda.device(dev):
-        out = torch.empty((B, L, ch), dtype=torch.float32, device=dev)
-        _lib.check(_lib.load().camal_act_read(
-            _lib.ptr(codes), _lib.ptr(scales), FORMATS[ckpt.fmt][1], B * L, ch, _lib.ptr(g), _lib.ptr(b),
-            int(bool(relu) and g is not None), *map(_lib.ptr, r), _lib.ptr(out), _stream(dev)))
+    out = torch.empty((B, L, ch), dtype=torch.float32, device=dev)
+    _call(dev, _lib.load().camal_act_read, codes.data_ptr(), scales.data_ptr(), FORMATS[ckpt.fmt][1], B * L, ch, _ptr(g), _ptr(b),
+          int(bool(relu) and g is not None), *map(_ptr, r), out.data_ptr())
     return out
 
 
@@ -158,13 +174,10 @@ def norm_backward(da, ckpt, invstd, gamma, beta, relu=True):
     da = _floats(da, (B, ch) if pooled else (B, L, ch), dev, "da")
     p = [_floats(t, (ch,), dev, n) for t, n in ((invstd, "invstd"), (gamma, "gamma"), (beta, "beta"))]
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        dz = torch.empty((B, L, ch), dtype=torch.float32, device=dev)
-        dgamma, dbeta = torch.empty((2, ch), dtype=torch.float32, device=dev)
-        ws = torch.empty(int(lib.camal_act_norm_bwd_workspace_bytes(B * L, ch)), dtype=torch.uint8, device=dev)
-        _lib.check(lib.camal_act_norm_bwd(
-            _lib.ptr(da), int(pooled), _lib.ptr(codes), _lib.ptr(scales), FORMATS[ckpt.fmt][1], B, L, ch, *map(_lib.ptr, p),
-            int(bool(relu)), _lib.ptr(dz), _lib.ptr(dgamma), _lib.ptr(dbeta), _lib.ptr(ws), ws.numel(), _stream(dev)))
+    dz, dgamma, dbeta = torch.empty((B, L, ch), dtype=torch.float32, device=dev), torch.empty_like(p[1]), torch.empty_like(p[1])
+    ws = torch.empty(lib.camal_act_norm_bwd_workspace_bytes(B * L, ch), dtype=torch.uint8, device=dev)
+    _call(dev, lib.camal_act_norm_bwd, da.data_ptr(), int(pooled), codes.data_ptr(), scales.data_ptr(), FORMATS[ckpt.fmt][1], B, L, ch,
+          *map(_ptr, p), int(bool(relu)), dz.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr(), ws.numel())
     return dz, dgamma, dbeta
 
 
@@ -185,10 +198,8 @@ def conv_weight_grad(dz, ckpt, kernel_size, gamma, beta, relu=True, skip=None, z
     g, b = _floats(gamma, (cin,), dev, "gamma"), _floats(beta, (cin,), dev, "beta")
     r = _skip(skip, ckpt)
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        dw = torch.empty((cout, cin, ks), dtype=torch.float32, device=dev)
-        ws = torch.empty(int(lib.camal_act_wgrad_workspace_bytes(B, L, cin, cout, ks)), dtype=torch.uint8, device=dev)
-        _lib.check(lib.camal_act_wgrad(
-            _lib.ptr(dz), _lib.ptr(codes), _lib.ptr(scales), FORMATS[ckpt.fmt][1], B, L, cin, cout, ks, _lib.ptr(g), _lib.ptr(b),
-            int(bool(relu)), *map(_lib.ptr, r), int(bool(zero_pad)), _lib.ptr(dw), _lib.ptr(ws), ws.numel(), _stream(dev)))
+    dw = torch.empty((cout, cin, ks), dtype=torch.float32, device=dev)
+    ws = torch.empty(lib.camal_act_wgrad_workspace_bytes(B, L, cin, cout, ks), dtype=torch.uint8, device=dev)
+    _call(dev, lib.camal_act_wgrad, dz.data_ptr(), codes.data_ptr(), scales.data_ptr(), FORMATS[ckpt.fmt][1], B, L, cin, cout, ks,
+          g.data_ptr(), b.data_ptr(), int(bool(relu)), *map(_ptr, r), int(bool(zero_pad)), dw.data_ptr(), ws.data_ptr(), ws.numel())
     return dw

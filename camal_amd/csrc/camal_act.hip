@@ -55,11 +55,20 @@ int act_check(std::initializer_list<const void*> floats, std::initializer_list<c
 
 inline int act_blocks(size_t work, size_t per_block, int cap) { return (int)std::min<size_t>((work + per_block - 1) / per_block, (size_t)cap); }
 
-inline size_t act_bwd_blocks(size_t rows) { return (rows + ACT_BWD_ROWS - 1) / ACT_BWD_ROWS; }
+// whether an fp32 output of n4 quads goes past the L3
+inline bool act_streams(size_t n4) { return n4 * 16 >= ACT_STREAM_BYTES; }
+
+inline size_t act_bwd_blocks(size_t rows) { return std::min<size_t>((rows + ACT_BWD_ROWS - 1) / ACT_BWD_ROWS, ACT_BWD_BLOCKS); }
 
 template <typename F, int C, bool RELU, bool BCAST>
 int act_norm_bwd_impl(hipStream_t s, const float* da, ActCodes k, const float* invstd, const float* gamma, const float* beta, int N,
                       int L, float* dz, float* dgamma, float* dbeta, void* ws) {
+    if (N <= ACT_SMALL_ROWS) {
+        hipLaunchKernelGGL((act_bwd_small_kernel<F, RELU, BCAST>), dim3(C / 32), dim3(1024), 0, s, da, k.codes, k.scales, invstd, gamma,
+                           beta, N, L, C, dz, dgamma, dbeta);
+        HIP_TRY(hipGetLastError());
+        return 0;
+    }
     const int nb = (int)act_bwd_blocks(N);
     double* partial = (double*)ws;
     float* means = (float*)(partial + (size_t)nb * C * 2);
@@ -69,7 +78,7 @@ int act_norm_bwd_impl(hipStream_t s, const float* da, ActCodes k, const float* i
     hipLaunchKernelGGL(act_bwd_final_kernel<C>, dim3(C / ACT_FINAL_CPB), dim3(ACT_FINAL_THREADS), 0, s, partial, nb, N, means,
                        dgamma, dbeta);
     hipLaunchKernelGGL((act_bwd_apply_kernel<F, C, RELU, BCAST>), dim3(act_blocks(n4, 256, 4096)), dim3(256), 0, s, da, k.codes,
-                       k.scales, invstd, gamma, beta, means, n4, L, dz);
+                       k.scales, invstd, gamma, beta, means, n4, L, act_streams(n4), dz);
     HIP_TRY(hipGetLastError());
     return 0;
 }
@@ -156,10 +165,13 @@ size_t camal::act_wgrad_max_bytes(int B, int L, int cin, int cout, int ks) {
 int camal::act_wgrad(hipStream_t s, const float* dz, const ActIn& in, int B, int L, int cin, int cout, int ks, float* dw,
                      float* bias_grad, float* part) {
     const ActPlan p = act_wgrad_plan(B, L, cin, cout, ks);
+    const bool direct = p.nsplit == 1;
+    float* sums = direct ? dw : part;
+    const ActOut out = direct ? ActOut{0, 1, cin * ks, ks} : ActOut{cout * cin * ks, cout * cin, cin, 1};
     const dim3 grid(p.nsplit, p.groups * (cin / (32 * p.ciw)), std::max(1, cout / 128));
     auto launch = [&](auto co, auto ciw, auto nt) {
         hipLaunchKernelGGL((act_wgrad_kernel<decltype(co)::value, decltype(ciw)::value, decltype(nt)::value>), grid,
-                           dim3(64 * ACT_WAVES), 0, s, dz, in, part, p.B, p.L, cin, ks, p.units, p.n_hi);
+                           dim3(64 * ACT_WAVES), 0, s, dz, in, sums, out, bias_grad, p.B, p.L, cin, ks, p.units, p.n_hi);
         return 0;
     };
     const int rc = with_channels(cout, [&](auto co) {
@@ -170,11 +182,13 @@ int camal::act_wgrad(hipStream_t s, const float* dz, const ActIn& in, int B, int
         return fail(CAMAL_ERR_STATE, "no weight-gradient kernel for this kernel size");
     });
     if (rc) return rc;
+    HIP_TRY(hipGetLastError());
+    if (direct) return 0;
     const int quads = cout * cin * ks / 4;
     if (quads >= 1 << 15 || p.nsplit <= 16)
-        hipLaunchKernelGGL(act_wgrad_reduce_kernel<4>, dim3((quads + 63) / 64), dim3(256), 0, s, part, p.nsplit, cout, cin, ks, dw, bias_grad);
+        hipLaunchKernelGGL(act_wgrad_reduce_kernel<4>, dim3((quads + 63) / 64), dim3(256), 0, s, part, p.nsplit, cout, cin, ks, dw);
     else
-        hipLaunchKernelGGL(act_wgrad_reduce_kernel<16>, dim3((quads + 15) / 16), dim3(256), 0, s, part, p.nsplit, cout, cin, ks, dw, bias_grad);
+        hipLaunchKernelGGL(act_wgrad_reduce_kernel<16>, dim3((quads + 15) / 16), dim3(256), 0, s, part, p.nsplit, cout, cin, ks, dw);
     HIP_TRY(hipGetLastError());
     return 0;
 }

@@ -191,7 +191,11 @@ __global__ __launch_bounds__(256) void act_read_kernel(const unsigned* __restric
 // ---- backward of norm + ReLU from the checkpoint -----------------------------------------------------------------------
 //   dy = da * [fma(x, gamma, beta) > 0],  s1 = sum dy,  s2 = sum dy x,  dz = gamma invstd (dy - s1/N - x s2/N)
 // The sums come first, so the input is read twice by nature.  BCAST: da[b][t][c] = dpool[b][c] / L.
-#define ACT_BWD_ROWS 64  // rows per workgroup of the first stage
+// First stage.  A block takes chunks of ACT_BWD_ROWS rows, one after another; a lane 4 channels of every G-th row of a chunk,
+// ACT_BWD_FLIGHT of them in flight.  fp32 sums run over a lane's rows of one chunk (at most 64) and are then carried in 64
+// bits; at most ACT_BWD_BLOCKS blocks, so that the second stage has little to read whatever the number of rows.
+#define ACT_BWD_ROWS 64
+#define ACT_BWD_BLOCKS 1024
 
 template <typename F, int C, bool RELU, bool BCAST>
 __global__ __launch_bounds__(256) void act_bwd_partial_kernel(const float* __restrict__ da, const unsigned* __restrict__ codes,
@@ -199,46 +203,51 @@ __global__ __launch_bounds__(256) void act_bwd_partial_kernel(const float* __res
                                                               const float* __restrict__ gamma, const float* __restrict__ beta,
                                                               int N, int L, double* __restrict__ partial) {
     constexpr int Q = C / 4, G = 256 / Q, RPL = ACT_BWD_ROWS / G;
-    __shared__ float sh[G][C][2];
+    __shared__ double sh[G][C][2];
     const int q4 = threadIdx.x % Q, c4 = q4 * 4, g = threadIdx.x / Q;
-    const int r0 = blockIdx.x * ACT_BWD_ROWS;
+    const int chunks = (N + ACT_BWD_ROWS - 1) / ACT_BWD_ROWS;
     float ga[4], be[4];
     load4(gamma + c4, ga); load4(beta + c4, be);
-    unsigned w[RPL], e[RPL];
-    float dv[RPL][4];
-#pragma unroll
-    for (int u = 0; u < RPL; ++u) {
-        const int r = r0 + g + u * G;
-        const int rc = r < N ? r : N - 1;  // a row past the end loads a valid address and counts for nothing
-        w[u] = codes[(size_t)rc * Q + q4];
-        e[u] = scales[(size_t)rc * (C / 32) + (q4 >> 3)];
-        load4(BCAST ? da + (size_t)(rc / L) * C + c4 : da + (size_t)rc * C + c4, dv[u]);
-    }
     const float len = (float)L;
-    float s1[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+    double t1[4] = {0., 0., 0., 0.}, t2[4] = {0., 0., 0., 0.};
+    for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+        const int r0 = chunk * ACT_BWD_ROWS + g;
+        unsigned w[RPL], e[RPL];
+        float dv[RPL][4];
 #pragma unroll
-    for (int u = 0; u < RPL; ++u) {
-        const bool live = r0 + g + u * G < N;
-        float x[4];
-        F::unpack(w[u], x);
-        const float s = act_scale(e[u]);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float xh = x[k] * s;
-            float d = BCAST ? dv[u][k] / len : dv[u][k];
-            if (RELU) d = fmaf(xh, ga[k], be[k]) > 0.f ? d : 0.f;
-            s1[k] += live ? d : 0.f;
-            s2[k] += live ? d * xh : 0.f;
+        for (int u = 0; u < RPL; ++u) {
+            const int rc = min(r0 + u * G, N - 1);  // a row past the end loads a valid address and counts for nothing
+            w[u] = codes[(size_t)rc * Q + q4];
+            e[u] = scales[(size_t)rc * (C / 32) + (q4 >> 3)];
+            load4(BCAST ? da + (size_t)(rc / L) * C + c4 : da + (size_t)rc * C + c4, dv[u]);
         }
+        float s1[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < RPL; ++u) {
+            const bool live = r0 + u * G < N;
+            float x[4];
+            F::unpack(w[u], x);
+            const float s = act_scale(e[u]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float xh = x[k] * s;
+                float d = BCAST ? dv[u][k] / len : dv[u][k];
+                if (RELU) d = fmaf(xh, ga[k], be[k]) > 0.f ? d : 0.f;
+                s1[k] += live ? d : 0.f;
+                s2[k] += live ? d * xh : 0.f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { t1[k] += (double)s1[k]; t2[k] += (double)s2[k]; }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) { sh[g][c4 + k][0] = s1[k]; sh[g][c4 + k][1] = s2[k]; }
+    for (int k = 0; k < 4; ++k) { sh[g][c4 + k][0] = t1[k]; sh[g][c4 + k][1] = t2[k]; }
     __syncthreads();
     if (threadIdx.x < C) {
         const int c = threadIdx.x;
         double a = 0.0, b = 0.0;
 #pragma unroll
-        for (int k = 0; k < G; ++k) { a += (double)sh[k][c][0]; b += (double)sh[k][c][1]; }
+        for (int k = 0; k < G; ++k) { a += sh[k][c][0]; b += sh[k][c][1]; }
         partial[((size_t)blockIdx.x * C + c) * 2 + 0] = a;
         partial[((size_t)blockIdx.x * C + c) * 2 + 1] = b;
     }
@@ -291,12 +300,22 @@ __global__ __launch_bounds__(ACT_FINAL_THREADS) void act_bwd_final_kernel(const 
     dgamma[c] = (float)b;
 }
 
+// A dz that the 256 MiB L3 cannot hold for its reader is stored past it (`stream`): left there, its lines are written out under
+// the next kernel's reads.  24 x 10080 x 256 (248 MB): 179 -> 150 us, all of it in the first stage's reads.  The same stores in
+// the write and read kernels change nothing (83.0 and 47.3 us either way on 124 and 189 MB).
+#define ACT_STREAM_BYTES (128u << 20)
+__device__ __forceinline__ void act_store4(float* p, const float (&o)[4], bool stream) {
+    const f32x4 v = {o[0], o[1], o[2], o[3]};
+    if (stream) __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(p));
+    else *reinterpret_cast<f32x4*>(p) = v;
+}
+
 template <typename F, int C, bool RELU, bool BCAST>
 __global__ __launch_bounds__(256) void act_bwd_apply_kernel(const float* __restrict__ da, const unsigned* __restrict__ codes,
                                                             const unsigned char* __restrict__ scales,
                                                             const float* __restrict__ invstd, const float* __restrict__ gamma,
                                                             const float* __restrict__ beta, const float* __restrict__ means,
-                                                            size_t n4, int L, float* __restrict__ dz) {
+                                                            size_t n4, int L, bool stream, float* __restrict__ dz) {
     constexpr int Q = C / 4;
     const int c = (int)(threadIdx.x % Q) * 4;
     float is[4], g[4], b[4], a1[4], a2[4];
@@ -312,7 +331,73 @@ __global__ __launch_bounds__(256) void act_bwd_apply_kernel(const float* __restr
             if (RELU) dy = fmaf(x[k], g[k], b[k]) > 0.f ? dy : 0.f;
             o[k] = g[k] * is[k] * (dy - a1[k] - x[k] * a2[k]);
         }
-        store4(dz + i * 4, o[0], o[1], o[2], o[3]);
+        act_store4(dz + i * 4, o, stream);
+    }
+}
+
+// All of it in one launch for at most ACT_SMALL_ROWS rows, where three launches cost more than the work: a workgroup has 32
+// channels (a scale block) and keeps its rows in registers between the sums and their use.  A call in a stream of calls /
+// alone: 14.7 / 28.1 us here and 19.5 / 31.2 us there at 384 rows, 14.8 / 30.7 at 1024, 15.8 / 38.2 at 2048 (32 to 256
+// channels alike).
+#define ACT_SMALL_ROWS 1024
+template <typename F, bool RELU, bool BCAST>
+__global__ __launch_bounds__(1024) void act_bwd_small_kernel(const float* __restrict__ da, const unsigned* __restrict__ codes,
+                                                             const unsigned char* __restrict__ scales,
+                                                             const float* __restrict__ invstd, const float* __restrict__ gamma,
+                                                             const float* __restrict__ beta, int N, int L, int C,
+                                                             float* __restrict__ dz, float* __restrict__ dgamma,
+                                                             float* __restrict__ dbeta) {
+    constexpr int U = ACT_SMALL_ROWS / 128;
+    __shared__ double sh[16][32][2];
+    __shared__ __align__(16) float mean[2][32];
+    const int q = threadIdx.x & 7, g = threadIdx.x >> 3, c = blockIdx.x * 32 + 4 * q, wave = threadIdx.x >> 6;
+    float ga[4], be[4], is[4];
+    load4(gamma + c, ga); load4(beta + c, be); load4(invstd + c, is);
+    const float len = (float)L;
+    float x[U][4], dy[U][4], s1[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (u * 128 >= N) break;
+        const int r = g + u * 128, rc = min(r, N - 1);
+        F::unpack(codes[(size_t)rc * (C / 4) + c / 4], x[u]);
+        const float s = act_scale(scales[(size_t)rc * (C / 32) + blockIdx.x]);
+        load4(da + (size_t)(BCAST ? rc / L : rc) * C + c, dy[u]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            x[u][k] *= s;
+            if (BCAST) dy[u][k] /= len;
+            if (RELU) dy[u][k] = fmaf(x[u][k], ga[k], be[k]) > 0.f ? dy[u][k] : 0.f;
+            s1[k] += r < N ? dy[u][k] : 0.f;
+            s2[k] += r < N ? dy[u][k] * x[u][k] : 0.f;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        double a = (double)s1[k], b = (double)s2[k];
+#pragma unroll
+        for (int m = 8; m < 64; m <<= 1) { a += __shfl_xor(a, m, 64); b += __shfl_xor(b, m, 64); }
+        if ((threadIdx.x & 63) < 8) { sh[wave][4 * q + k][0] = a; sh[wave][4 * q + k][1] = b; }
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        const int ch = threadIdx.x & 31, which = threadIdx.x >> 5;
+        double a = 0.0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) a += sh[w][ch][which];
+        mean[which][ch] = (float)(a / N);
+        (which ? dgamma : dbeta)[blockIdx.x * 32 + ch] = (float)a;
+    }
+    __syncthreads();
+    float a1[4], a2[4];
+    load4(&mean[0][4 * q], a1); load4(&mean[1][4 * q], a2);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (u * 128 >= N) break;
+        const int r = g + u * 128;
+        float o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = ga[k] * is[k] * (dy[u][k] - a1[k] - x[u][k] * a2[k]);
+        if (r < N) store4(dz + (size_t)r * C + c, o[0], o[1], o[2], o[3]);
     }
 }
 
@@ -353,10 +438,15 @@ template <int COUT, int CIW, int NTAP> struct ActTile {
     static constexpr int BYTES = 2 * WK * 2 * TILE > CHUNK * SUMS ? 2 * WK * 2 * TILE : CHUNK * SUMS;
 };
 
+// Where the sums go, in floats: partial sums [split][tap][co][ci], or with one split the gradient [co][ci][tap] itself
+struct ActOut {
+    int split, tap, co, ci;
+};
+
 template <int COUT, int CIW, int NTAP>
 __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float* __restrict__ dz, const ActIn& in,
-                                               float* __restrict__ part, int B, int L, int cin, int ks, int units_per_split,
-                                               int j0) {
+                                               float* __restrict__ part, ActOut out, int B, int L, int cin, int ks,
+                                               int units_per_split, int j0) {
     using T = ActTile<COUT, CIW, NTAP>;
     constexpr int CO = T::CO, WK = T::WK;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave / CO, col = wave % CO;
@@ -565,7 +655,7 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
             if (owner == wk)
 #pragma unroll
                 for (int n = n0; n < n0 + CHUNK && n < TRIOS; ++n) {
-                    float* po = part + ((size_t)(blockIdx.x * ks + j0 + n / CIW) * COUT + co0 + 4 * h) * cin + ci0 + 32 * (n % CIW) + i;
+                    float* po = part + (size_t)blockIdx.x * out.split + (j0 + n / CIW) * out.tap + (co0 + 4 * h) * out.co + (ci0 + 32 * (n % CIW) + i) * out.ci;
 #pragma unroll
                     for (int k = 0; k < OWN / V; ++k) {
                         fv v;
@@ -577,7 +667,7 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
 #pragma unroll
                         for (int c = 0; c < V; ++c) {
                             const int reg = owner * OWN + k * V + c;
-                            po[(size_t)((reg & 3) + 8 * (reg >> 2)) * cin] = v[c];
+                            po[((reg & 3) + 8 * (reg >> 2)) * out.co] = v[c];
                         }
                     }
                 }
@@ -587,24 +677,26 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
 // grid = (splits, tap groups x ci tiles, groups of CO co tiles); the first n_hi tap groups take NHI taps, the others NHI - 1
 template <int COUT, int CIW, int NHI>
 __global__ __launch_bounds__(64 * ACT_WAVES, 2) void act_wgrad_kernel(const float* __restrict__ dz, ActIn in, float* __restrict__ part,
-                                                                      int B, int L, int cin, int ks, int units_per_split, int n_hi) {
+                                                                      ActOut out, float* __restrict__ bias_grad, int B, int L,
+                                                                      int cin, int ks, int units_per_split, int n_hi) {
     using T = ActTile<COUT, CIW, NHI>;
     __shared__ __align__(16) unsigned short lds[T::BYTES / 2];
     const int y = blockIdx.y / (cin / (32 * CIW));
+    if (bias_grad && blockIdx.x + blockIdx.y + blockIdx.z == 0 && threadIdx.x < COUT) bias_grad[threadIdx.x] = 0.f;
     if (y < n_hi) {
-        act_wgrad_body<COUT, CIW, NHI>(lds, dz, in, part, B, L, cin, ks, units_per_split, y * NHI);
+        act_wgrad_body<COUT, CIW, NHI>(lds, dz, in, part, out, B, L, cin, ks, units_per_split, y * NHI);
     } else {
         if constexpr (NHI > 1)
-            act_wgrad_body<COUT, CIW, NHI - 1>(lds, dz, in, part, B, L, cin, ks, units_per_split, n_hi * NHI + (y - n_hi) * (NHI - 1));
+            act_wgrad_body<COUT, CIW, NHI - 1>(lds, dz, in, part, out, B, L, cin, ks, units_per_split, n_hi * NHI + (y - n_hi) * (NHI - 1));
     }
 }
 
-// dw[co][ci][j] = sum_split part[split][j][co][ci]; bias_grad[0..cout) = 0 unless null.  Four ci per lane; the splits are dealt
+// dw[co][ci][j] = sum_split part[split][j][co][ci].  Four ci per lane; the splits are dealt
 // to GRP groups of lanes, each with independent 16-byte loads, combined in a fixed order.  A small dw needs many groups to
 // have enough loads in flight.
 template <int GRP>
 __global__ __launch_bounds__(256) void act_wgrad_reduce_kernel(const float* __restrict__ part, int nsplit, int cout, int cin, int ks,
-                                                               float* __restrict__ dw, float* __restrict__ bias_grad) {
+                                                               float* __restrict__ dw) {
     constexpr int QB = 256 / GRP;
     __shared__ float4 red[GRP][QB];
     const int total = cout * cin * ks;
@@ -633,7 +725,6 @@ __global__ __launch_bounds__(256) void act_wgrad_reduce_kernel(const float* __re
         o[2 * ks] = a.z;
         o[3 * ks] = a.w;
     }
-    if (bias_grad && blockIdx.x == 0 && threadIdx.x < cout) bias_grad[threadIdx.x] = 0.f;
 }
 
 }  // namespace camal

@@ -77,8 +77,11 @@ int act_norm_bwd_impl(hipStream_t s, const float* da, ActCodes k, const float* i
                        L, partial);
     hipLaunchKernelGGL(act_bwd_final_kernel<C>, dim3(C / ACT_FINAL_CPB), dim3(ACT_FINAL_THREADS), 0, s, partial, nb, N, means,
                        dgamma, dbeta);
-    hipLaunchKernelGGL((act_bwd_apply_kernel<F, C, RELU, BCAST>), dim3(act_blocks(n4, 256, 4096)), dim3(256), 0, s, da, k.codes,
-                       k.scales, invstd, gamma, beta, means, n4, L, act_streams(n4), dz);
+    with_flag(act_streams(n4), [&](auto st) {
+        hipLaunchKernelGGL((act_bwd_apply_kernel<F, C, RELU, BCAST, decltype(st)::value>), dim3(act_blocks(n4, 256, 4096)), dim3(256), 0,
+                           s, da, k.codes, k.scales, invstd, gamma, beta, means, n4, L, dz);
+        return 0;
+    });
     HIP_TRY(hipGetLastError());
     return 0;
 }

@@ -300,22 +300,23 @@ __global__ __launch_bounds__(ACT_FINAL_THREADS) void act_bwd_final_kernel(const 
     dgamma[c] = (float)b;
 }
 
-// A dz that the 256 MiB L3 cannot hold for its reader is stored past it (`stream`): left there, its lines are written out under
+// A dz that the 256 MiB L3 cannot hold for its reader is stored past it (STREAM): left there, its lines are written out under
 // the next kernel's reads.  24 x 10080 x 256 (248 MB): 179 -> 150 us, all of it in the first stage's reads.  The same stores in
 // the write and read kernels change nothing (83.0 and 47.3 us either way on 124 and 189 MB).
 #define ACT_STREAM_BYTES (128u << 20)
-__device__ __forceinline__ void act_store4(float* p, const float (&o)[4], bool stream) {
+template <bool STREAM>
+__device__ __forceinline__ void act_store4(float* p, const float (&o)[4]) {  // (a run-time choice: hipcc merges the two stores)
     const f32x4 v = {o[0], o[1], o[2], o[3]};
-    if (stream) __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(p));
+    if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(p));
     else *reinterpret_cast<f32x4*>(p) = v;
 }
 
-template <typename F, int C, bool RELU, bool BCAST>
+template <typename F, int C, bool RELU, bool BCAST, bool STREAM>
 __global__ __launch_bounds__(256) void act_bwd_apply_kernel(const float* __restrict__ da, const unsigned* __restrict__ codes,
                                                             const unsigned char* __restrict__ scales,
                                                             const float* __restrict__ invstd, const float* __restrict__ gamma,
                                                             const float* __restrict__ beta, const float* __restrict__ means,
-                                                            size_t n4, int L, bool stream, float* __restrict__ dz) {
+                                                            size_t n4, int L, float* __restrict__ dz) {
     constexpr int Q = C / 4;
     const int c = (int)(threadIdx.x % Q) * 4;
     float is[4], g[4], b[4], a1[4], a2[4];
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(256) void act_bwd_apply_kernel(const float* __restr
             if (RELU) dy = fmaf(x[k], g[k], b[k]) > 0.f ? dy : 0.f;
             o[k] = g[k] * is[k] * (dy - a1[k] - x[k] * a2[k]);
         }
-        act_store4(dz + i * 4, o, stream);
+        act_store4<STREAM>(dz + i * 4, o);
     }
 }
 

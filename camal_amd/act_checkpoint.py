@@ -71,9 +71,9 @@ def _rows(t):
 
 
 def _floats(t, shape, device, name):
-    if not torch.is_tensor(t) or t.dtype != torch.float32 or tuple(t.shape) != tuple(shape) or t.device != device:
+    if not torch.is_tensor(t) or t.dtype != torch.float32 or t.shape != shape or t.device != device:
         raise ValueError(f"{name}: expected a float32 tensor of shape {tuple(shape)} on {device}")
-    return _rows(t)
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else _rows(t)
 
 
 def _ckpt(c, device, name, shape=None, fmt=None):
@@ -130,11 +130,13 @@ def write(z, mean, invstd, gamma, beta, relu=True, fmt="int8", skip=None):
         raise ValueError(f"z is [windows, time, channels] with channels in {CHANNELS}")
     dev, (B, L, ch) = _device(z), z.shape
     dtype, code = FORMATS[fmt]
-    a = [_floats(z, z.shape, dev, "z")] + [_floats(t, (ch,), dev, n) for t, n in zip((mean, invstd, gamma, beta), ("mean", "invstd", "gamma", "beta"))]
+    n = (ch,)
+    a = [_floats(z, z.shape, dev, "z"), _floats(mean, n, dev, "mean"), _floats(invstd, n, dev, "invstd"),
+         _floats(gamma, n, dev, "gamma"), _floats(beta, n, dev, "beta")]
     r = [None] * 5
     if skip is not None:
         names = ("skip z", "skip mean", "skip invstd", "skip gamma", "skip beta")
-        r = [_floats(t, s, dev, n) for t, s, n in zip(skip, (z.shape, *((ch,),) * 4), names, strict=True)]
+        r = [_floats(t, s, dev, name) for t, s, name in zip(skip, (z.shape, n, n, n, n), names, strict=True)]
     out, kept = torch.empty_like(a[0]), _new(a[0], dtype)
     if skip is None:
         _call(dev, _lib.load().camal_act_write, *map(_ptr, a), int(bool(relu)), *r, B * L, ch, code, out.data_ptr(),

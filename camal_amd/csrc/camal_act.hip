@@ -4,7 +4,6 @@
 #include "camal_act_kernels.hpp"
 
 #include <algorithm>
-#include <climits>
 #include <initializer_list>
 #include <type_traits>
 
@@ -37,7 +36,7 @@ int with_channels(int c, Fn&& f) {
 // What the entry points share: the shape, null pointers, alignment of the float rows (16-byte loads) and of the rest (4-byte)
 int act_check(std::initializer_list<const void*> floats, std::initializer_list<const void*> words,
               std::initializer_list<const void*> bytes, long long rows, int channels, int format) {
-    if (rows < 1 || rows > INT_MAX) return fail(CAMAL_ERR_ARG, "the number of rows must be in 1 .. 2^31 - 1");
+    if (rows < 1 || rows > ACT_MAX_ROWS) return fail(CAMAL_ERR_ARG, "the number of rows must be in 1 .. 2^31 - 4096");
     if (!act_channels_ok(channels)) return fail(CAMAL_ERR_ARG, "channels must be 32, 64, 128 or 256");
     if (!act_format_ok(format)) return fail(CAMAL_ERR_ARG, "format must be CAMAL_ACT_INT8 or CAMAL_ACT_E4M3");
     for (const void* p : floats) {
@@ -226,7 +225,7 @@ int camal_act_read(const void* codes, const unsigned char* scales, int format, l
 }
 
 size_t camal_act_norm_bwd_workspace_bytes(long long rows, int channels) {
-    return rows < 1 || rows > INT_MAX || !act_channels_ok(channels) ? 0 : act_norm_bwd_bytes((size_t)rows, channels);
+    return rows < 1 || rows > ACT_MAX_ROWS || !act_channels_ok(channels) ? 0 : act_norm_bwd_bytes((size_t)rows, channels);
 }
 
 int camal_act_norm_bwd(const float* da, int pooled, const void* codes, const unsigned char* scales, int format, int B, int L,
@@ -242,7 +241,7 @@ int camal_act_norm_bwd(const float* da, int pooled, const void* codes, const uns
 }
 
 static bool act_wgrad_shape_ok(int B, int L, int cin, int cout, int ks) {
-    return B >= 1 && L >= 1 && (long long)B * L <= INT_MAX && act_channels_ok(cin) && act_channels_ok(cout) && ks >= 1 && ks <= 63 && (ks & 1);
+    return B >= 1 && L >= 1 && (long long)B * L <= ACT_MAX_ROWS && act_channels_ok(cin) && act_channels_ok(cout) && ks >= 1 && ks <= 63 && (ks & 1);
 }
 
 size_t camal_act_wgrad_workspace_bytes(int B, int L, int cin, int cout, int ks) {

@@ -5,6 +5,9 @@
 
 namespace camal {
 
+// rows of one call: row indices are 32-bit and run up to a tile past the last
+constexpr long long ACT_MAX_ROWS = (1LL << 31) - 4096;
+
 // A train-mode BatchNorm: batch statistics, scale and shift
 struct ActNorm {
     const float *mean, *invstd, *gamma, *beta;

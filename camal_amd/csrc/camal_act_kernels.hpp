@@ -426,7 +426,6 @@ __global__ __launch_bounds__(1024) void act_bwd_small_kernel(const float* __rest
 #define ACT_TAPS 8    // taps a wave takes at most
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 // How a workgroup is made up, and the passes in which the CO waves of a unit fill its input tile (4 channels per lane)
 template <int COUT, int CIW, int NTAP> struct ActTile {

@@ -3,8 +3,6 @@
 // (reference src/helpers/torch_trainer.py:281-298): forward in train() mode (BatchNorm batch
 // statistics), mean cross-entropy, backward, AdamW.
 #pragma once
-#include <climits>
-
 #include "camal_act.hpp"
 #include "camal_train_kernels.hpp"
 
@@ -380,8 +378,8 @@ int camal_trainer_create_act(int device_id, int kernel_size, int max_batch, int 
     if (!out) return fail(CAMAL_ERR_ARG, "null argument");
     if (act_format != CAMAL_ACT_NONE && act_format != CAMAL_ACT_INT8 && act_format != CAMAL_ACT_E4M3)
         return fail(CAMAL_ERR_ARG, "act_format must be CAMAL_ACT_NONE, CAMAL_ACT_INT8 or CAMAL_ACT_E4M3");
-    if (act_format != CAMAL_ACT_NONE && (long long)max_batch * max_len > INT_MAX)
-        return fail(CAMAL_ERR_ARG, "max_batch * max_len must be below 2^31");
+    if (act_format != CAMAL_ACT_NONE && (long long)max_batch * max_len > ACT_MAX_ROWS)
+        return fail(CAMAL_ERR_ARG, "max_batch * max_len must be at most 2^31 - 4096");
     if (!mid_supported(mid_channels)) return fail(CAMAL_ERR_ARG, "mid_channels must be 32, 64 or 128");
     const int C2 = 2 * mid_channels;  // this model's widest layer (shadows the default)
     if (arch != CAMAL_ARCH_CAMAL && arch != CAMAL_ARCH_RESNET) return fail(CAMAL_ERR_ARG, "arch must be 0 (CamALResNet) or 1 (ResNet)");

@@ -332,7 +332,7 @@ int camal_trainer_peek(camal_trainer* t, int what, int index, int B, int L, floa
  * ReLU than fma(x, gamma, beta), the neighbour on x's side is taken: the backward pass has the forward pass's mask
  * exactly (gamma and beta must be the ones the checkpoint was written with).
  *
- * channels in {32, 64, 128, 256}; 1 <= rows < 2^31.  float tensors 16-byte aligned, codes 4-byte aligned; inputs and
+ * channels in {32, 64, 128, 256}; 1 <= rows <= 2^31 - 4096.  float tensors 16-byte aligned, codes 4-byte aligned; inputs and
  * outputs must not overlap.  All calls are asynchronous on `stream`, on the current device, allocate nothing and may be
  * captured into a graph; results do not depend on scheduling.  Calls that can overlap need workspaces of their own. */
 /* Normalise, ReLU (relu != 0), add the skip branch, and keep:
@@ -365,7 +365,7 @@ int camal_act_norm_bwd(const float* da_dev, int pooled, const void* codes_dev, c
  *   a = bf16([relu](fma(x, gamma, beta)) [+ fma(x_r, gamma_r, beta_r)])
  * The activation enters with the 8 significant bits of bf16 (its code has at most 7); dz enters with all of its 24 and
  * the products are summed in fp32.  dz_dev [B][L][cout] fp32, dw [cout][cin][ks] fp32.  cin, cout in {32, 64, 128, 256},
- * ks <= 63.  An infinite dz gives NaN.                                                                             */
+ * ks <= 63.  An infinite dz gives NaN.  A NaN in the last ks/2 rows of a window may reach every tap of its channel.  */
 size_t camal_act_wgrad_workspace_bytes(int B, int L, int cin, int cout, int ks); /* 0 if unsupported */
 int camal_act_wgrad(const float* dz_dev, const void* codes_dev, const unsigned char* scales_dev, int format, int B, int L, int cin,
                     int cout, int ks, const float* gamma, const float* beta, int relu, const void* codes_r_dev,

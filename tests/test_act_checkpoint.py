@@ -421,6 +421,40 @@ def test_captured_and_replayed():
 
 
 @gpu
+def test_offsets_beyond_32_bits():
+    """2.2e9 elements: the last rows come out as in a call of their own."""
+    from camal_amd import act_checkpoint as ac
+    rows, ch, tail = 8_600_000, 256, 70
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GB of GPU memory")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    z = torch.zeros(1, rows, ch, device="cuda")
+    z[:, -tail:] = torch.randn(1, tail, ch, device="cuda", generator=g)
+    n = _dev(torch.zeros(ch), torch.ones(ch), *_norm(ch, 5, torch.zeros(1, 4, ch))[2:])
+    out, ckpt = ac.write(z, *n, fmt="e4m3")
+    few, own = ac.write(z[:, -tail:], *n, fmt="e4m3")
+    assert torch.equal(out[:, -tail:], few) and torch.equal(ckpt.scales[:, -tail:], own.scales)
+    assert torch.equal(ckpt.codes[:, -tail:].view(torch.uint8), own.codes.view(torch.uint8))
+    assert torch.equal(ac.read(ckpt)[:, -tail:], ac.read(own))
+    del out
+    z.zero_()
+    z[:, -tail:] = torch.randn(1, tail, ch, device="cuda", generator=g)  # now the gradient: all in the last rows
+    dz, dgamma, dbeta = ac.norm_backward(z, ckpt, *n[1:])
+    kept = _values(own)
+    wz, wg, wb, m = ref.norm_backward(z[:, -tail:].cpu(), kept, *(t.cpu() for t in n[1:]))
+    t1, t2, _ = _bwd_tolerance(m, kept)
+    assert ((dbeta.cpu().double() - wb).abs() <= t1).all() and ((dgamma.cpu().double() - wg).abs() <= t2).all()
+    side = (n[2] * n[1] * torch.where(ac.read(own) * n[2] + n[3] > 0, z[:, -tail:], 0.0))
+    assert (dz[:, -tail:] - side).abs().max() <= 1e-4 * side.abs().max()  # the means are 1e-7 of it: 1.2e5 times fewer rows
+    del dz
+    dw = ac.conv_weight_grad(z, ckpt, 3, *n[2:])
+    a = ref.operand(kept, *(t.cpu() for t in n[2:]))
+    base = ref.operand(torch.zeros(1, 1, ch, dtype=torch.float64), *(t.cpu() for t in n[2:]))
+    want, mag = ref.weight_grad(torch.cat([torch.zeros(1, 1, ch), z[:, -tail:].cpu()], 1), torch.cat([base, a], 1), 3)
+    assert ((dw.cpu().double() - want).abs() <= (3 * tail + 8) * U * mag * 1.01).all()
+
+
+@gpu
 def test_rows_behind_the_last_stay_as_they_were():
     """The C entry points write exactly rows * channels elements."""
     from camal_amd import _lib

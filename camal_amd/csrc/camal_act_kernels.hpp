@@ -195,7 +195,7 @@ __global__ __launch_bounds__(256) void act_read_kernel(const unsigned* __restric
 // ACT_BWD_FLIGHT of them in flight.  fp32 sums run over a lane's rows of one chunk (at most 64) and are then carried in 64
 // bits; at most ACT_BWD_BLOCKS blocks, so that the second stage has little to read whatever the number of rows.
 #define ACT_BWD_ROWS 64
-#define ACT_BWD_BLOCKS 1024
+#define ACT_BWD_BLOCKS 512
 
 template <typename F, int C, bool RELU, bool BCAST>
 __global__ __launch_bounds__(256) void act_bwd_partial_kernel(const float* __restrict__ da, const unsigned* __restrict__ codes,

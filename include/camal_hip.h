@@ -365,7 +365,7 @@ int camal_act_norm_bwd(const float* da_dev, int pooled, const void* codes_dev, c
  *   a = bf16([relu](fma(x, gamma, beta)) [+ fma(x_r, gamma_r, beta_r)])
  * The activation enters with the 8 significant bits of bf16 (its code has at most 7); dz enters with all of its 24 and
  * the products are summed in fp32.  dz_dev [B][L][cout] fp32, dw [cout][cin][ks] fp32.  cin, cout in {32, 64, 128, 256},
- * ks <= 63.  An infinite dz gives NaN.  A NaN in the last ks/2 rows of a window may reach every tap of its channel.  */
+ * ks <= 63.  An infinite dz gives NaN; a NaN in the input may reach every tap of its channel.                      */
 size_t camal_act_wgrad_workspace_bytes(int B, int L, int cin, int cout, int ks); /* 0 if unsupported */
 int camal_act_wgrad(const float* dz_dev, const void* codes_dev, const unsigned char* scales_dev, int format, int B, int L, int cin,
                     int cout, int ks, const float* gamma, const float* beta, int relu, const void* codes_r_dev,

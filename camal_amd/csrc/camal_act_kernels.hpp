@@ -428,8 +428,8 @@ __global__ __launch_bounds__(1024) void act_bwd_small_kernel(const float* __rest
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // How a workgroup is made up, and the passes in which the CO waves of a unit fill its input tile (4 channels per lane)
-template <int COUT, int CIW, int NTAP> struct ActTile {
-    static constexpr int CO = COUT >= 128 ? 4 : COUT / 32, WK = ACT_WAVES / CO;
+template <int CO, int CIW, int NTAP> struct ActTile {
+    static constexpr int WK = ACT_WAVES / CO;
     static constexpr int RPW = 8 / CIW, RPP = RPW * CO, ROWS = (ACT_UNIT + NTAP + 6) / 8 * 8, PASS = (ROWS + RPP - 1) / RPP;
     static constexpr int TILE = CIW * ROWS * 32;  // halfwords
     // LDS: two tiles per unit, then the waves' sums: ACT_WAVES * (16 - 16 / WK) registers per accumulator, CHUNK of them at once
@@ -443,12 +443,12 @@ struct ActOut {
     int split, tap, co, ci;
 };
 
-template <int COUT, int CIW, int NTAP>
+template <int COUT, int CO, int CIW, int NTAP>
 __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float* __restrict__ dz, const ActIn& in,
                                                float* __restrict__ part, ActOut out, int B, int L, int cin, int ks,
                                                int units_per_split, int j0) {
-    using T = ActTile<COUT, CIW, NTAP>;
-    constexpr int CO = T::CO, WK = T::WK;
+    using T = ActTile<CO, CIW, NTAP>;
+    constexpr int WK = T::WK;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave / CO, col = wave % CO;
     const int i = lane & 31, h = lane >> 5, co0 = (blockIdx.z * CO + col) * 32, ci0 = blockIdx.y % (cin / (32 * CIW)) * 32 * CIW;
     const int tpw = (L + ACT_UNIT - 1) / ACT_UNIT, total = B * tpw;
@@ -675,19 +675,19 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
 }
 
 // grid = (splits, tap groups x ci tiles, groups of CO co tiles); the first n_hi tap groups take NHI taps, the others NHI - 1
-template <int COUT, int CIW, int NHI>
+template <int COUT, int CO, int CIW, int NHI>
 __global__ __launch_bounds__(64 * ACT_WAVES, 2) void act_wgrad_kernel(const float* __restrict__ dz, ActIn in, float* __restrict__ part,
                                                                       ActOut out, float* __restrict__ bias_grad, int B, int L,
                                                                       int cin, int ks, int units_per_split, int n_hi) {
-    using T = ActTile<COUT, CIW, NHI>;
+    using T = ActTile<CO, CIW, NHI>;
     __shared__ __align__(16) unsigned short lds[T::BYTES / 2];
     const int y = blockIdx.y / (cin / (32 * CIW));
     if (bias_grad && blockIdx.x + blockIdx.y + blockIdx.z == 0 && threadIdx.x < COUT) bias_grad[threadIdx.x] = 0.f;
     if (y < n_hi) {
-        act_wgrad_body<COUT, CIW, NHI>(lds, dz, in, part, out, B, L, cin, ks, units_per_split, y * NHI);
+        act_wgrad_body<COUT, CO, CIW, NHI>(lds, dz, in, part, out, B, L, cin, ks, units_per_split, y * NHI);
     } else {
         if constexpr (NHI > 1)
-            act_wgrad_body<COUT, CIW, NHI - 1>(lds, dz, in, part, out, B, L, cin, ks, units_per_split, n_hi * NHI + (y - n_hi) * (NHI - 1));
+            act_wgrad_body<COUT, CO, CIW, NHI - 1>(lds, dz, in, part, out, B, L, cin, ks, units_per_split, n_hi * NHI + (y - n_hi) * (NHI - 1));
     }
 }
 

@@ -91,7 +91,6 @@ int act_norm_bwd_impl(hipStream_t s, const float* da, ActCodes k, const float* i
 // CO = co tiles of a workgroup: 4 share the decoding of their input best, 2 leave half the partial sums.  The latter wins
 // where a wave has few units (128 out-channels; us with 4 / with 2): 25 taps on 37 x 333, 4 units a wave, 34.7 / 31.4; 7 taps
 // on 128 x 510, 8 units, 45.2 / 44.7; 7 taps, 256 channels on 8 x 10080, 40 units, 177 / 186.
-struct ActPlan { int B, L, ciw, co, groups, n_hi, nhi, nsplit, units, want; };
 ActPlan act_wgrad_plan(int B, int L, int cin, int cout, int ks) {
     ActPlan p;
     p.B = ks == 1 ? 1 : B;  // one tap knows no window edges
@@ -100,7 +99,7 @@ ActPlan act_wgrad_plan(int B, int L, int cin, int cout, int ks) {
     const int base = ks / p.groups, rem = ks % p.groups;
     p.nhi = rem ? base + 1 : base;
     p.n_hi = rem ? rem : p.groups;
-    p.ciw = cin >= 64 && p.nhi <= 4 ? 2 : 1;
+    p.ciw = cin >= 64 && cout >= 64 && p.nhi <= 4 ? 2 : 1;  // 32 out-channels: nobody shares the decoding, the codes fill the registers
     const int total = p.B * ((p.L + ACT_UNIT - 1) / ACT_UNIT);
     auto cut = [&](int co) {
         const int tiles = p.groups * (cin / (32 * p.ciw)) * (cout / (32 * co)), wk = ACT_WAVES / co;
@@ -177,27 +176,8 @@ int camal::act_wgrad(hipStream_t s, const float* dz, const ActIn& in, int B, int
     const bool direct = p.nsplit == 1;
     float* sums = direct ? dw : part;
     const ActOut out = direct ? ActOut{0, 1, cin * ks, ks} : ActOut{cout * cin * ks, cout * cin, cin, 1};
-    const dim3 grid(p.nsplit, p.groups * (cin / (32 * p.ciw)), cout / (32 * p.co));
-    auto launch = [&](auto cc, auto co, auto ciw, auto nt) {
-        hipLaunchKernelGGL((act_wgrad_kernel<decltype(cc)::value, decltype(co)::value, decltype(ciw)::value, decltype(nt)::value>), grid,
-                           dim3(64 * ACT_WAVES), 0, s, dz, in, sums, out, bias_grad, p.B, p.L, cin, ks, p.units, p.n_hi);
-        return 0;
-    };
-    auto with_taps = [&](auto cc, auto co) {
-#define CAMAL_ACT_WG(W, N) if (p.ciw == W && p.nhi == N) return launch(cc, co, std::integral_constant<int, W>(), std::integral_constant<int, N>());
-        CAMAL_ACT_WG(1, 1) CAMAL_ACT_WG(1, 3) CAMAL_ACT_WG(1, 5) CAMAL_ACT_WG(1, 6) CAMAL_ACT_WG(1, 7) CAMAL_ACT_WG(1, 8)
-        CAMAL_ACT_WG(2, 1) CAMAL_ACT_WG(2, 3)
-#undef CAMAL_ACT_WG
-        return fail(CAMAL_ERR_STATE, "no weight-gradient kernel for this kernel size");
-    };
-    const int rc = with_channels(cout, [&](auto cc) {
-        constexpr int C = decltype(cc)::value;
-        if constexpr (C >= 128)
-            if (p.co == 2) return with_taps(cc, std::integral_constant<int, 2>());
-        return with_taps(cc, std::integral_constant<int, (C >= 128 ? 4 : C / 32)>());
-    });
-    if (rc) return rc;
-    HIP_TRY(hipGetLastError());
+    const auto launch = p.co == 4 ? act_wgrad_launch<4> : (p.co == 2 ? act_wgrad_launch<2> : act_wgrad_launch<1>);
+    if (int r = launch(s, p, dz, in, sums, out, bias_grad, cin, cout, ks)) return r;
     if (direct) return 0;
     const int quads = cout * cin * ks / 4;
     if (quads >= 1 << 15 || p.nsplit <= 16)

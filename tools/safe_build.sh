@@ -12,5 +12,5 @@ if ! python3 "$R/tools/check_ring.py" "$ASM" | tail -3; then
   echo "ring checker: findings -- not building $OUT"; rm -f "$ASM"; exit 1
 fi
 rm -f "$ASM"
-/opt/rocm/bin/hipcc $FLAGS -fPIC -shared "$@" -o "$OUT" "$R/camal_amd/csrc/camal_hip.hip" "$R/camal_amd/csrc/camal_act.hip"
+/opt/rocm/bin/hipcc $FLAGS -fPIC -shared "$@" -o "$OUT" "$R/camal_amd/csrc/camal_hip.hip" "$R"/camal_amd/csrc/camal_act*.hip
 echo "built $OUT"

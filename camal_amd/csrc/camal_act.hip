@@ -86,8 +86,9 @@ int act_norm_bwd_impl(hipStream_t s, const float* da, ActCodes k, const float* i
 }
 
 // How the weight gradient is cut up, fixed by the shapes alone: the sums have the same order on every call.
-// Tap groups of nearly equal size (9 = 5 + 4, 25 = 7 + 6 + 6 + 6); CIW = 32-wide ci tiles per wave: two where few taps leave
-// room for the accumulators, so that the pieces of dz serve more products; splits for one workgroup on each of 256 CUs.
+// Tap groups of nearly equal size (9 = 5 + 4, 25 = 7 + 6 + 6 + 6); splits for one workgroup on each of 256 CUs.  (Two ci tiles
+// a wave, which halves the cutting of dz, is slower where the taps leave room for it: 3 taps on 128 x 510, 128 -> 128 channels
+// 31.0 instead of 27.8 us, 64 -> 64 19.2 instead of 16.0.)
 // CO = co tiles of a workgroup: 4 share the decoding of their input best, 2 leave half the partial sums.  The latter wins
 // where a wave has few units (128 out-channels; us with 4 / with 2): 25 taps on 37 x 333, 4 units a wave, 34.7 / 31.4; 7 taps
 // on 128 x 510, 8 units, 45.2 / 44.7; 7 taps, 256 channels on 8 x 10080, 40 units, 177 / 186.
@@ -99,10 +100,9 @@ ActPlan act_wgrad_plan(int B, int L, int cin, int cout, int ks) {
     const int base = ks / p.groups, rem = ks % p.groups;
     p.nhi = rem ? base + 1 : base;
     p.n_hi = rem ? rem : p.groups;
-    p.ciw = cin >= 64 && cout >= 64 && p.nhi <= 4 ? 2 : 1;  // 32 out-channels: nobody shares the decoding, the codes fill the registers
     const int total = p.B * ((p.L + ACT_UNIT - 1) / ACT_UNIT);
     auto cut = [&](int co) {
-        const int tiles = p.groups * (cin / (32 * p.ciw)) * (cout / (32 * co)), wk = ACT_WAVES / co;
+        const int tiles = p.groups * (cin / 32) * (cout / (32 * co)), wk = ACT_WAVES / co;
         p.co = co;
         p.want = std::min(std::max(1, 256 / tiles), (total + wk - 1) / wk);
         p.units = (total + p.want - 1) / p.want;
@@ -180,10 +180,7 @@ int camal::act_wgrad(hipStream_t s, const float* dz, const ActIn& in, int B, int
     if (int r = launch(s, p, dz, in, sums, out, bias_grad, cin, cout, ks)) return r;
     if (direct) return 0;
     const int quads = cout * cin * ks / 4;
-    if (quads >= 1 << 15 || p.nsplit <= 16)
-        hipLaunchKernelGGL(act_wgrad_reduce_kernel<4>, dim3((quads + 63) / 64), dim3(256), 0, s, part, p.nsplit, cout, cin, ks, dw);
-    else
-        hipLaunchKernelGGL(act_wgrad_reduce_kernel<16>, dim3((quads + 15) / 16), dim3(256), 0, s, part, p.nsplit, cout, cin, ks, dw);
+    hipLaunchKernelGGL(act_wgrad_reduce_kernel, dim3((quads + 15) / 16), dim3(256), 0, s, part, p.nsplit, cout, cin, ks, dw);
     HIP_TRY(hipGetLastError());
     return 0;
 }

@@ -26,10 +26,9 @@ struct ActIn {
     int e4m3, relu, zero_pad;
 };
 
-// How the weight gradient is cut up: windows B of L steps (one tap: all rows as one window), CIW ci tiles per wave and CO co
-// tiles per workgroup, tap groups (the first n_hi take nhi taps, the others nhi - 1), splits of `units` units each.  want =
+// How the weight gradient is cut up: windows B of L steps (one tap: all rows as one window), CO co tiles per workgroup, tap groups (the first n_hi take nhi taps, the others nhi - 1), splits of `units` units each.  want =
 // the splits aimed at, at least nsplit
-struct ActPlan { int B, L, ciw, co, groups, n_hi, nhi, nsplit, units, want; };
+struct ActPlan { int B, L, co, groups, n_hi, nhi, nsplit, units, want; };
 #define ACT_UNIT 64   // timesteps of a unit
 #define ACT_WAVES 8   // waves of a workgroup
 // Taps a wave takes at most: with 8 the accumulators of one tile leave too few registers (23 to 71 spilled).  15 taps as

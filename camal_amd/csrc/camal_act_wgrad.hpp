@@ -15,7 +15,7 @@ namespace camal {
 //   a holds 8 significant bits (the code behind it has 7 or 4), so it is a bf16 operand without loss.  dz is cut into three
 //   bf16 pieces, each the leading 8 bits of what is left: they add up to it exactly, so the three products, summed in the
 //   instruction's fp32, are an fp32 product sum at a third of the bf16 rate, 5 times the rate of fp32 MFMA.
-// One wave = 32 co x CIW * 32 ci x NTAP taps on a unit of 64 timesteps.  The 8 waves of a workgroup are CO co tiles x WK units:
+// One wave = 32 co x 32 ci x NTAP taps on a unit of 64 timesteps.  The 8 waves of a workgroup are CO co tiles x WK units:
 // the CO waves of a unit share its decoded input, and the WK sums of a tile are added in LDS before they leave the workgroup
 // (what the partial sums weigh is what bounds a short call).
 //   A: dz straight from global memory into registers, as the fragment wants it: no other wave needs these values; rows past
@@ -34,37 +34,35 @@ namespace camal {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // How a workgroup is made up, and the passes in which the CO waves of a unit fill its input tile (4 channels per lane)
-template <int CO, int CIW, int NTAP> struct ActTile {
+template <int CO, int NTAP> struct ActTile {
     static constexpr int WK = ACT_WAVES / CO;
-    static constexpr int RPW = 8 / CIW, RPP = RPW * CO, ROWS = (ACT_UNIT + NTAP + 6) / 8 * 8, PASS = (ROWS + RPP - 1) / RPP;
-    static constexpr int TILE = CIW * ROWS * 32;  // halfwords
+    static constexpr int RPP = 8 * CO, ROWS = (ACT_UNIT + NTAP + 6) / 8 * 8, PASS = (ROWS + RPP - 1) / RPP;
+    static constexpr int TILE = ROWS * 32;  // halfwords
     // LDS: two tiles per unit, then the waves' sums: ACT_WAVES * (16 - 16 / WK) registers per accumulator, CHUNK of them at once
     static constexpr int SUMS = ACT_WAVES * (16 - 16 / WK) * 64 * 4, FIT = 128 * 1024 / SUMS;
-    static constexpr int CHUNK = NTAP * CIW < FIT ? NTAP * CIW : FIT;
+    static constexpr int CHUNK = NTAP < FIT ? NTAP : FIT;
     static constexpr int BYTES = 2 * WK * 2 * TILE > CHUNK * SUMS ? 2 * WK * 2 * TILE : CHUNK * SUMS;
 };
 
-template <int CO, int CIW, int NTAP>
+template <int CO, int NTAP>
 __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float* __restrict__ dz, const ActIn& in,
                                                float* __restrict__ part, ActOut out, int B, int L, int cin, int cout,
                                                int ks, int units_per_split, int j0) {
-    using T = ActTile<CO, CIW, NTAP>;
+    using T = ActTile<CO, NTAP>;
     constexpr int WK = T::WK;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave / CO, col = wave % CO;
-    const int i = lane & 31, h = lane >> 5, co0 = (blockIdx.z * CO + col) * 32, ci0 = blockIdx.y % (cin / (32 * CIW)) * 32 * CIW;
+    const int i = lane & 31, h = lane >> 5, co0 = (blockIdx.z * CO + col) * 32, ci0 = blockIdx.y % (cin / 32) * 32;
     const int tpw = (L + ACT_UNIT - 1) / ACT_UNIT, total = B * tpw;
     const int lo = min(total, (int)blockIdx.x * units_per_split), hi = min(total, lo + units_per_split);
 
-    f32x16 acc[NTAP][CIW];
+    f32x16 acc[NTAP];
 #pragma unroll
     for (int j = 0; j < NTAP; ++j)
 #pragma unroll
-        for (int w = 0; w < CIW; ++w)
-#pragma unroll
-            for (int k = 0; k < 16; ++k) acc[j][w][k] = 0.f;
+        for (int k = 0; k < 16; ++k) acc[j][k] = 0.f;
 
     // ---- the input tile: a lane has 4 channels of every RPP-th row ----
-    const int cq = lane % (8 * CIW), r0 = col * T::RPW + lane / (8 * CIW), lgc = 31 - __builtin_clz(cin);
+    const int cq = lane % 8, r0 = col * 8 + lane / 8, lgc = 31 - __builtin_clz(cin);
     float g[4], b[4], gr[4] = {0.f, 0.f, 0.f, 0.f}, br[4] = {0.f, 0.f, 0.f, 0.f};
     load4(in.gamma + ci0 + 4 * cq, g); load4(in.beta + ci0 + 4 * cq, b);
     if (in.codes_r) { load4(in.gamma_r + ci0 + 4 * cq, gr); load4(in.beta_r + ci0 + 4 * cq, br); }
@@ -89,9 +87,9 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
         return o;
     };
     auto fetch = [&](const Source& o, int p) {
-        if (col * T::RPW + p * T::RPP >= T::ROWS) return;
+        if (col * 8 + p * T::RPP >= T::ROWS) return;
         const int rel = max(-o.rb, min(o.tb - o.rb + r0 + p * T::RPP, L - 1 - o.rb));
-        const int oc = (rel << lgc) + ci0 + 4 * cq, os = (rel << (lgc - 5)) + ci0 / 32 + cq / 8;
+        const int oc = (rel << lgc) + ci0 + 4 * cq, os = (rel << (lgc - 5)) + ci0 / 32;
         cw[p] = __builtin_amdgcn_raw_buffer_load_b32(o.codes, oc, 0, 0);
         cs[p] = __builtin_amdgcn_raw_buffer_load_b8(o.scales, os, 0, 0);
         if (in.codes_r) {
@@ -100,7 +98,7 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
         }
     };
     auto stash = [&](unsigned short* tile, int tb, int p) {
-        if (col * T::RPW + p * T::RPP >= T::ROWS) return;
+        if (col * 8 + p * T::RPP >= T::ROWS) return;
         float a[4];
         if (in.e4m3) ActE4M3::unpack(cw[p], a); else ActI8::unpack(cw[p], a);
         const float sc = act_scale(cs[p]);
@@ -119,7 +117,7 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
 #pragma unroll
             for (int k = 0; k < 4; ++k) a[k] = inside ? a[k] : 0.f;
         }
-        *reinterpret_cast<uint2*>(tile + ((cq / 8) * T::ROWS + row) * 32 + 4 * (cq % 8)) = make_uint2(pk_bf16(a[0], a[1]), pk_bf16(a[2], a[3]));
+        *reinterpret_cast<uint2*>(tile + row * 32 + 4 * cq) = make_uint2(pk_bf16(a[0], a[1]), pk_bf16(a[2], a[3]));
     };
 
     // ---- dz: 8 times of this lane's channel per step, loaded two steps before it is cut, cut a step before it is used ----
@@ -146,11 +144,10 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
 
     // ---- the B operand: lane's place in a transposing read is rows 8 h + (l % 16) / 4 (+ 4), channels 16 ((l / 16) & 1) +
     // 4 (l % 4) .. + 3 ----
-    constexpr int TRIOS = NTAP * CIW;
     const int bp = (8 * h + (lane & 15) / 4) * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    auto operand = [&](const unsigned short* tile, int s, int n) {  // trio n = tap * CIW + ci tile
+    auto operand = [&](const unsigned short* tile, int s, int tap) {
         typedef __attribute__((address_space(3))) s16x4 lds4;
-        const unsigned short* q = tile + bp + ((n % CIW) * T::ROWS + 16 * s + n / CIW) * 32;
+        const unsigned short* q = tile + bp + (16 * s + tap) * 32;
         const s16x4 b0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)q);
         const s16x4 b1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(q + 4 * 32));
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -202,17 +199,16 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
                 // idle (the two waves of a SIMD share it evenly, reach their clumps together and overlap nothing).
                 constexpr int STASH = (T::PASS + 3) / 4, TASKS = 5 + STASH;
 #pragma unroll
-                for (int n = 0; n < TRIOS; ++n) {
+                for (int n = 0; n < NTAP; ++n) {
                     bf16x8 bn;
-                    if (n + 1 < TRIOS) bn = operand(now, s, n + 1);
+                    if (n + 1 < NTAP) bn = operand(now, s, n + 1);
                     else if (s < 3) bn = operand(now, s + 1, 0);
 #pragma unroll
                     for (int p = 2; p >= 0; --p)
-                        acc[n / CIW][n % CIW] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, pc[s & 1][p]), bt,
-                                                                                       acc[n / CIW][n % CIW], 0, 0, 0);
+                        acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, pc[s & 1][p]), bt, acc[n], 0, 0, 0);
 #pragma unroll
                     for (int t = 0; t < TASKS; ++t) {
-                        if (t * TRIOS / TASKS != n) continue;
+                        if (t * NTAP / TASKS != n) continue;
                         if (t < 4) cut(s + 1, t);
                         else if (t == 4) { if (s == 0) load_dz(dsrc, 3); else load_dz(dnext, s - 1); }
                         else {
@@ -226,7 +222,7 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
             dsrc = dnext;
         }
     }
-    // acc[j][w][reg] of lane l: row co = co0 + (reg & 3) + 8 (reg >> 2) + 4 h, column ci = ci0 + 32 w + i.  Of a tile's 16
+    // acc[j][reg] of lane l: row co = co0 + (reg & 3) + 8 (reg >> 2) + 4 h, column ci = ci0 + i.  Of a tile's 16
     // registers each of its WK waves adds OWN and hands the others out through LDS, as many tiles at once as fit: the
     // workgroup has the CU to itself.
     constexpr int OWN = 16 / WK, V = OWN < 4 ? OWN : 4, CHUNK = T::CHUNK;
@@ -236,10 +232,10 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
         return ((((tile * WK + owner) * (WK - 1) + (from < owner ? from : from - 1)) * CO + col) * (OWN / V) + k) * 64 + lane;
     };
 #pragma unroll
-    for (int n0 = 0; n0 < TRIOS; n0 += CHUNK) {
+    for (int n0 = 0; n0 < NTAP; n0 += CHUNK) {
         __syncthreads();
 #pragma unroll
-        for (int n = n0; n < n0 + CHUNK && n < TRIOS; ++n)
+        for (int n = n0; n < n0 + CHUNK && n < NTAP; ++n)
 #pragma unroll
             for (int owner = 0; owner < WK; ++owner)
                 if (owner != wk)
@@ -247,7 +243,7 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
                     for (int k = 0; k < OWN / V; ++k) {
                         fv v;
 #pragma unroll
-                        for (int c = 0; c < V; ++c) v[c] = acc[n / CIW][n % CIW][owner * OWN + k * V + c];
+                        for (int c = 0; c < V; ++c) v[c] = acc[n][owner * OWN + k * V + c];
                         red[slot(n - n0, owner, wk, k)] = v;
                     }
         __syncthreads();
@@ -255,13 +251,13 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
         for (int owner = 0; owner < WK; ++owner)
             if (owner == wk)
 #pragma unroll
-                for (int n = n0; n < n0 + CHUNK && n < TRIOS; ++n) {
-                    float* po = part + (size_t)blockIdx.x * out.split + (j0 + n / CIW) * out.tap + (co0 + 4 * h) * out.co + (ci0 + 32 * (n % CIW) + i) * out.ci;
+                for (int n = n0; n < n0 + CHUNK && n < NTAP; ++n) {
+                    float* po = part + (size_t)blockIdx.x * out.split + (j0 + n) * out.tap + (co0 + 4 * h) * out.co + (ci0 + i) * out.ci;
 #pragma unroll
                     for (int k = 0; k < OWN / V; ++k) {
                         fv v;
 #pragma unroll
-                        for (int c = 0; c < V; ++c) v[c] = acc[n / CIW][n % CIW][owner * OWN + k * V + c];
+                        for (int c = 0; c < V; ++c) v[c] = acc[n][owner * OWN + k * V + c];
 #pragma unroll
                         for (int from = 0; from < WK; ++from)
                             if (from != owner) v += red[slot(n - n0, owner, from, k)];
@@ -276,38 +272,41 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
 }
 
 // grid = (splits, tap groups x ci tiles, groups of CO co tiles); the first n_hi tap groups take NHI taps, the others NHI - 1
-template <int CO, int CIW, int NHI>
+template <int CO, int NHI>
 __global__ __launch_bounds__(64 * ACT_WAVES, 2) void act_wgrad_kernel(const float* __restrict__ dz, ActIn in, float* __restrict__ part,
                                                                       ActOut out, float* __restrict__ bias_grad, int B, int L,
                                                                       int cin, int cout, int ks, int units_per_split,
                                                                       int n_hi) {
-    using T = ActTile<CO, CIW, NHI>;
+    using T = ActTile<CO, NHI>;
     __shared__ __align__(16) unsigned short lds[T::BYTES / 2];
-    const int y = blockIdx.y / (cin / (32 * CIW));
+    const int y = blockIdx.y / (cin / 32);
     if (bias_grad && blockIdx.x + blockIdx.y + blockIdx.z == 0 && threadIdx.x < cout) bias_grad[threadIdx.x] = 0.f;
     if (y < n_hi) {
-        act_wgrad_body<CO, CIW, NHI>(lds, dz, in, part, out, B, L, cin, cout, ks, units_per_split, y * NHI);
+        act_wgrad_body<CO, NHI>(lds, dz, in, part, out, B, L, cin, cout, ks, units_per_split, y * NHI);
     } else {
         if constexpr (NHI > 1)
-            act_wgrad_body<CO, CIW, NHI - 1>(lds, dz, in, part, out, B, L, cin, cout, ks, units_per_split, n_hi * NHI + (y - n_hi) * (NHI - 1));
+            act_wgrad_body<CO, NHI - 1>(lds, dz, in, part, out, B, L, cin, cout, ks, units_per_split, n_hi * NHI + (y - n_hi) * (NHI - 1));
     }
 }
 
-// The kernel for the plan's tap groups and ci tiles
+// The kernel for the plan's tap groups
 template <int CO>
 int act_wgrad_launch(hipStream_t s, const ActPlan& p, const float* dz, const ActIn& in, float* sums, ActOut out, float* bias_grad, int cin,
                      int cout, int ks) {
-    const dim3 grid(p.nsplit, p.groups * (cin / (32 * p.ciw)), cout / (32 * CO));
-    auto launch = [&](auto ciw, auto taps) {
-        hipLaunchKernelGGL((act_wgrad_kernel<CO, decltype(ciw)::value, decltype(taps)::value>), grid, dim3(64 * ACT_WAVES), 0, s, dz, in,
-                           sums, out, bias_grad, p.B, p.L, cin, cout, ks, p.units, p.n_hi);
+    const dim3 grid(p.nsplit, p.groups * (cin / 32), cout / (32 * CO));
+    auto launch = [&](auto taps) {
+        hipLaunchKernelGGL((act_wgrad_kernel<CO, decltype(taps)::value>), grid, dim3(64 * ACT_WAVES), 0, s, dz, in, sums, out, bias_grad,
+                           p.B, p.L, cin, cout, ks, p.units, p.n_hi);
         HIP_TRY(hipGetLastError());
         return 0;
     };
-#define CAMAL_ACT_WG(W, N) if (p.ciw == W && p.nhi == N) return launch(std::integral_constant<int, W>(), std::integral_constant<int, N>());
-    CAMAL_ACT_WG(1, 1) CAMAL_ACT_WG(1, 3) CAMAL_ACT_WG(1, 5) CAMAL_ACT_WG(1, 6) CAMAL_ACT_WG(1, 7)
-    if constexpr (CO > 1) { CAMAL_ACT_WG(2, 1) CAMAL_ACT_WG(2, 3) }
-#undef CAMAL_ACT_WG
+    switch (p.nhi) {
+        case 1: return launch(std::integral_constant<int, 1>());
+        case 3: return launch(std::integral_constant<int, 3>());
+        case 5: return launch(std::integral_constant<int, 5>());
+        case 6: return launch(std::integral_constant<int, 6>());
+        case 7: return launch(std::integral_constant<int, 7>());
+    }
     return fail(CAMAL_ERR_STATE, "no weight-gradient kernel for this kernel size");
 }
 

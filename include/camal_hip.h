@@ -253,7 +253,7 @@ size_t camal_trainer_param_count_widths(int kernel_size, int arch, int mid_chann
 size_t camal_trainer_running_count_widths(int mid_channels);                          /* 0 if unsupported */
 /* The same with 8-bit activation checkpoints (below): act_format CAMAL_ACT_INT8 or CAMAL_ACT_E4M3 keeps the forward pass for
  * the backward pass in one byte per element, CAMAL_ACT_NONE in fp32 (the calls above).  The forward pass, the loss and the
- * ReLU masks are the same bit for bit; the gradients see the normalised activations as the codes hold them.  With
+ * ReLU masks are the same bit for bit (but a NaN passes the ReLU here); the gradients see the normalised activations as the codes hold them.  With
  * mid_channels 64 a timestep takes 3.8 KB of workspace instead of 11.1 KB.                                       */
 #define CAMAL_ACT_NONE (-1)
 #define CAMAL_ACT_INT8 0

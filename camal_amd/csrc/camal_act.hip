@@ -89,9 +89,9 @@ int act_norm_bwd_impl(hipStream_t s, const float* da, ActCodes k, const float* i
 // Tap groups of nearly equal size (9 = 5 + 4, 25 = 7 + 6 + 6 + 6); splits for one workgroup on each of 256 CUs.  (Two ci tiles
 // a wave, which halves the cutting of dz, is slower where the taps leave room for it: 3 taps on 128 x 510, 128 -> 128 channels
 // 31.0 instead of 27.8 us, 64 -> 64 19.2 instead of 16.0.)
-// CO = co tiles of a workgroup: 4 share the decoding of their input best, 2 leave half the partial sums.  The latter wins
-// where a wave has few units (128 out-channels; us with 4 / with 2): 25 taps on 37 x 333, 4 units a wave, 34.7 / 31.4; 7 taps
-// on 128 x 510, 8 units, 45.2 / 44.7; 7 taps, 256 channels on 8 x 10080, 40 units, 177 / 186.
+// CO = co tiles of a workgroup, as many as there are up to 4: they share the decoding of their input.  (Two of four tiles leave
+// half the partial sums: 25 taps on 37 x 333 33.4 instead of 34.4 us, but 20.7 instead of 20.3 for one tap on 128 x 510 and 186
+// instead of 177 for 7 taps on 8 x 10080.)
 ActPlan act_wgrad_plan(int B, int L, int cin, int cout, int ks) {
     ActPlan p;
     p.B = ks == 1 ? 1 : B;  // one tap knows no window edges
@@ -101,15 +101,11 @@ ActPlan act_wgrad_plan(int B, int L, int cin, int cout, int ks) {
     p.nhi = rem ? base + 1 : base;
     p.n_hi = rem ? rem : p.groups;
     const int total = p.B * ((p.L + ACT_UNIT - 1) / ACT_UNIT);
-    auto cut = [&](int co) {
-        const int tiles = p.groups * (cin / 32) * (cout / (32 * co)), wk = ACT_WAVES / co;
-        p.co = co;
-        p.want = std::min(std::max(1, 256 / tiles), (total + wk - 1) / wk);
-        p.units = (total + p.want - 1) / p.want;
-        p.nsplit = (total + p.units - 1) / p.units;  // at most want, which grows with B and L
-        return (p.units + wk - 1) / wk;              // units of a wave
-    };
-    if (cut(std::min(4, cout / 32)) <= 6 && cout >= 128) cut(2);
+    p.co = std::min(4, cout / 32);
+    const int tiles = p.groups * (cin / 32) * (cout / (32 * p.co)), wk = ACT_WAVES / p.co;
+    p.want = std::min(std::max(1, 256 / tiles), (total + wk - 1) / wk);
+    p.units = (total + p.want - 1) / p.want;
+    p.nsplit = (total + p.units - 1) / p.units;  // at most want, which grows with B and L
     return p;
 }
 

@@ -26,9 +26,10 @@ namespace camal {
 // On these SIMDs a vector instruction hides behind a matrix product only up to about three per product (measured: 15.9 ns a
 // product alone, 16.3 with 2, 18.1 with 4, 23.3 with 8 vector instructions to each, two waves), so what counts beside the
 // products is the number of vector instructions: cutting dz takes 44 per 21 products of 7 taps, decoding is shared.
-// 256 -> 256 channels, 7 taps, 8 x 10080: 173 us, 1290 TF of bf16 products (MFMA busy 0.71, the clock at 1.74 GHz under this load;
-// a large library product reaches 1130 TF here); 128 -> 128, 7 taps, 128 x 510: 43 us, of which about 7 until the first product,
-// 25 in the products, 6 in writing 29 MB of sums at the end, and 6 more in the second stage.  With two pieces of dz instead
+// 256 -> 256 channels, 7 taps, 8 x 10080: 173 to 180 us, 1240 to 1290 TF of bf16 products (MFMA busy 0.71, the clock at 1.74 GHz under this load;
+// a large library product reaches 1130 TF here); 128 -> 128, 7 taps, 128 x 510: 43 us (and 6 of the
+// second stage), of which about 7 until the first product,
+// 25 in the products and 6 in writing 29 MB of sums at the end.  With two pieces of dz instead
 // of three: 0.8 of the time, error 2.5e-6 instead of 3e-7 (norm-wise): not taken.
 // Each split's sums go to part[split][j][co][ci]; act_wgrad_reduce_kernel adds them in a fixed order.
 typedef short s16x4 __attribute__((ext_vector_type(4)));

@@ -398,6 +398,39 @@ def test_strides_offsets_and_streams():
 
 
 @gpu
+def test_two_streams_at_once():
+    """Calls that overlap on two streams have workspaces of their own: the same results as one after the other."""
+    from camal_amd import act_checkpoint as ac
+    sets = [_inputs(B=16, L=300, seed=60), _inputs(B=9, L=510, ch=128, cout=64, seed=70)]
+    want = [_run_all(ac, *i[0], *i[1:]) for i in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k, (st, i) in enumerate(zip(streams, sets)):
+            with torch.cuda.stream(st):
+                got[k].append(_run_all(ac, *i[0], *i[1:]))
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        assert all(torch.equal(a, b) for r in runs for a, b in zip(w, r))
+
+
+@gpu
+def test_sliced_and_turned_checkpoints():
+    """A slice of a checkpoint (its scales start at any byte) and one whose memory is laid out otherwise."""
+    from camal_amd import act_checkpoint as ac
+    (z, _), n, _, da, dz = _inputs(B=5, L=33, ch=32)
+    _, ckpt = ac.write(z, *n, fmt="e4m3")
+    _, few = ac.write(z[1:4], *n, fmt="e4m3")
+    want = [ac.read(few), *ac.norm_backward(da[1:4], few, *n[1:]), ac.conv_weight_grad(dz[1:4], few, 3, *n[2:])]
+    turn = lambda t: t.view(torch.uint8).transpose(0, 1).contiguous().transpose(0, 1).view(t.dtype)  # noqa: E731
+    for c in (ac.ActivationCheckpoint(ckpt.codes[1:4], ckpt.scales[1:4]),
+              ac.ActivationCheckpoint(turn(few.codes), turn(few.scales))):
+        got = [ac.read(c), *ac.norm_backward(da[1:4], c, *n[1:]), ac.conv_weight_grad(dz[1:4], c, 3, *n[2:])]
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@gpu
 def test_captured_and_replayed():
     """Two graphs of the whole run, replayed in turns with new inputs and eager work in between."""
     from camal_amd import act_checkpoint as ac

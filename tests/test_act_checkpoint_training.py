@@ -100,7 +100,7 @@ def _backward64(eng, x, y, feat, kept, invstd, params):
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("k,B,L,arch,mid", [(7, 5, 64, "camal", 64), (25, 3, 97, "camal", 64), (5, 4, 33, "camal", 32),
                                             (9, 2, 70, "camal", 128), (7, 3, 81, "resnet", 64), (3, 37, 5, "camal", 64),
-                                            (15, 1, 200, "camal", 32), (63, 2, 40, "camal", 64)])
+                                            (15, 1, 200, "camal", 32), (63, 2, 40, "camal", 64), (7, 1, 1, "camal", 64)])
 def test_step_against_a_64_bit_backward_on_the_checkpoints(k, B, L, arch, mid, fmt):
     from camal_amd import synth
     from camal_amd.trainer import TrainEngine

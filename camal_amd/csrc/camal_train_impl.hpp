@@ -535,8 +535,10 @@ int train_bwd_impl(camal_trainer* t, const float* params, const float* x, const 
     const TLayout& Y = t->lay;
     const int N = B * L;
     int r;
-    // head + loss
-    hipLaunchKernelGGL(head_loss_kernel<C2>, dim3(B), dim3(HEAD_LOSS_THREADS), 0, s, t->act[8], params + Y.wfc, params + Y.bfc,
+    // head + loss.  With checkpoints the features live in gA, which a backward pass overwrites: a caller's dlogits (its first
+    // or a further one for this batch) go with the means that the forward pass left in `pooled`.
+    const float* feat = ext_dlogits && t->ckpt() ? nullptr : t->act[8];
+    hipLaunchKernelGGL(head_loss_kernel<C2>, dim3(B), dim3(HEAD_LOSS_THREADS), 0, s, feat, params + Y.wfc, params + Y.bfc,
                        y ? y : (const int*)t->correct, B, L, t->grad_scale, t->pooled, t->dpool, t->logits, t->dlogits, t->loss, t->correct,
                        ext_dlogits);
     HIP_TRY(hipGetLastError());

@@ -323,7 +323,7 @@ __global__ __launch_bounds__(256) void bn_bwd_apply_kernel(const float* __restri
 // gradient of the caller's loss with respect to the logits, [B][2], used in place of the cross-entropy's.
 #define HEAD_LOSS_THREADS 1024
 template <int C>  // C = 2 mid_channels: the feature width the head sees
-__global__ __launch_bounds__(HEAD_LOSS_THREADS) void head_loss_kernel(const float* __restrict__ feat /*[B][L][C]*/,
+__global__ __launch_bounds__(HEAD_LOSS_THREADS) void head_loss_kernel(const float* __restrict__ feat /*[B][L][C]; null: `pooled` is given*/,
                                                         const float* __restrict__ wfc, const float* __restrict__ bfc,
                                                         const int* __restrict__ labels, int B, int L, float grad_scale,
                                                         float* __restrict__ pooled /*[B][C]*/,
@@ -336,20 +336,25 @@ __global__ __launch_bounds__(HEAD_LOSS_THREADS) void head_loss_kernel(const floa
     __shared__ float sl[4];
     constexpr int TG = HEAD_LOSS_THREADS / C;  // time groups per channel
     const int b = blockIdx.x, c = threadIdx.x % C, tg = threadIdx.x / C;
-    const float* f = feat + (size_t)b * L * C;
-    float s = 0.f;
+    if (feat) {
+        const float* f = feat + (size_t)b * L * C;
+        float s = 0.f;
 #pragma unroll 4
-    for (int t = tg; t < L; t += TG) s += f[(size_t)t * C + c];
-    sp[threadIdx.x] = s;
-    __syncthreads();
-    if (threadIdx.x < C) {
-        float a = 0.f;
+        for (int t = tg; t < L; t += TG) s += f[(size_t)t * C + c];
+        sp[threadIdx.x] = s;
+        __syncthreads();
+        if (threadIdx.x < C) {
+            float a = 0.f;
 #pragma unroll
-        for (int k = 0; k < TG; ++k) a += sp[c + C * k];
-        sp[c] = a / (float)L;
+            for (int k = 0; k < TG; ++k) a += sp[c + C * k];
+            sp[c] = a / (float)L;
+        }
+        __syncthreads();
+        if (threadIdx.x < C) pooled[(size_t)b * C + c] = sp[c];
+    } else {
+        if (threadIdx.x < C) sp[c] = pooled[(size_t)b * C + c];
+        __syncthreads();
     }
-    __syncthreads();
-    if (threadIdx.x < C) pooled[(size_t)b * C + c] = sp[c];
     if (threadIdx.x < 2) {
         float a = 0.f;
         for (int k = 0; k < C; ++k) a = fmaf(wfc[threadIdx.x * C + k], sp[k], a);

@@ -294,7 +294,7 @@ int camal_train_fwd_bwd(camal_trainer* t, const float* params_dev, float* bn_run
  *      grads_dev exactly as camal_train_fwd_bwd writes them for the cross-entropy.
  * y_dev: labels for the accuracy count (NULL: ncorrect is meaningless); loss_dev receives the batch's mean
  * cross-entropy when y_dev is given (the caller's own loss value is the caller's).  No other call on this trainer
- * may come between steps 1 and 3.                                                                                */
+ * may come between steps 1 and 3.  Step 3 may be repeated with other dlogits of the same batch.                   */
 int camal_train_bwd_dlogits(camal_trainer* t, const float* params_dev, const float* x_dev, const int* y_dev,
                             const float* dlogits_dev, int B, int L, float* grads_dev, float* loss_dev, int* ncorrect_dev,
                             void* stream);

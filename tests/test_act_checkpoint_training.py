@@ -241,3 +241,35 @@ def test_peek_and_create_refusals():
     assert lib.camal_trainer_workspace_bytes(None) == 0
     full.close()
     eng.close()
+
+
+@gpu
+@pytest.mark.parametrize("fmt,mid,B,L", [(None, 64, 5, 70), ("int8", 64, 5, 70), ("e4m3", 32, 3, 41), ("int8", 128, 2, 130)])
+def test_one_forward_pass_serves_several_backward_passes(fmt, mid, B, L):
+    """Gradients of several losses of one batch: each is what a forward pass of its own gives, bit for bit, whatever ran
+    backward before it."""
+    from camal_amd import _lib, synth
+    from camal_amd.trainer import TrainEngine
+    eng = TrainEngine(_model(7, "camal", mid), "cuda:0", B, L, act_checkpoint=fmt)
+    x, y = synth.ideal_windows(B, L, seed=9)
+    x, y = torch.as_tensor(x).float().cuda().contiguous(), torch.as_tensor(y).int().cuda().contiguous()
+    g = torch.Generator().manual_seed(1)
+    losses = [torch.randn(B, 2, generator=g).cuda() / B for _ in range(3)]
+
+    def backward(dlogits):
+        _lib.check(eng.lib.camal_train_bwd_dlogits(eng._h, _lib.ptr(eng.params), _lib.ptr(x), _lib.ptr(y), _lib.ptr(dlogits), B, L,
+                                                   _lib.ptr(eng.grads), _lib.ptr(eng.loss), _lib.ptr(eng.ncorrect), eng._stream()))
+        return eng.grads.clone(), eng.loss.clone()
+
+    own = []
+    for d in losses:
+        eng.forward_train(x)
+        own.append(backward(d))
+    eng.forward_train(x)
+    for _ in range(2):
+        for d, want in zip(losses, own):
+            got = backward(d)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    eng.forward_backward(x, y, update_running=False)  # a whole step is a forward pass, too
+    assert torch.equal(backward(losses[0])[0], own[0][0])
+    eng.close()

@@ -89,6 +89,12 @@ int act_norm_bwd_impl(hipStream_t s, const float* da, ActCodes k, const float* i
 // Tap groups of nearly equal size (9 = 5 + 4, 25 = 7 + 6 + 6 + 6); splits for one workgroup on each of 256 CUs.  (Two ci tiles
 // a wave, which halves the cutting of dz, is slower where the taps leave room for it: 3 taps on 128 x 510, 128 -> 128 channels
 // 31.0 instead of 27.8 us, 64 -> 64 19.2 instead of 16.0.)
+// A long call gets gx of them at a time, one set after the other (the tiles of a set read the same rows), so that a wave's chain of
+// fp32 sums stays near ACT_CHAIN_ROWS rows: twice that at most, where long and short units alternate.  A matrix product cuts its
+// sum off instead of rounding it, an error of one sign that grows with the chain: dz and input of one sign, 100 x 10080, 256 -> 256
+// channels, 63 taps 1.3e-4 in one chain and 2.6e-6 here (a plain fp32 product 2.0e-6).  us, one set of longer chains / sets of
+// 8192 / 4096 rows: that case 24600 / 17430 / 17840 (one set leaves CUs idle); 7 taps, 400 x 10080, 128 -> 128: 1957 / 2024 / 2064;
+// 3 taps, 800 x 10080, 256 -> 256: 9480 / 9260 / 9330.
 // CO = co tiles of a workgroup, as many as there are up to 4: they share the decoding of their input.  (Two of four tiles leave
 // half the partial sums: 25 taps on 37 x 333 33.4 instead of 34.4 us, but 20.7 instead of 20.3 for one tap on 128 x 510 and 186
 // instead of 177 for 7 taps on 8 x 10080.)
@@ -103,9 +109,13 @@ ActPlan act_wgrad_plan(int B, int L, int cin, int cout, int ks) {
     const int total = p.B * ((p.L + ACT_UNIT - 1) / ACT_UNIT);
     p.co = std::min(4, cout / 32);
     const int tiles = p.groups * (cin / 32) * (cout / (32 * p.co)), wk = ACT_WAVES / p.co;
-    p.want = std::min(std::max(1, 256 / tiles), (total + wk - 1) / wk);
+    p.gx = std::min(std::max(1, 256 / tiles), (total + wk - 1) / wk);
+    const long long rows = (long long)p.gx * wk * ACT_CHAIN_ROWS;
+    p.want = p.gx * (int)(((long long)p.B * p.L + rows - 1) / rows);
     p.units = (total + p.want - 1) / p.want;
-    p.nsplit = (total + p.units - 1) / p.units;  // at most want, which grows with B and L
+    p.nsplit = (total + p.units - 1) / p.units;
+    if (p.want == p.gx) p.gx = p.nsplit;
+    p.nsplit = (p.nsplit + p.gx - 1) / p.gx * p.gx;  // at most want, which never falls as B and L grow
     return p;
 }
 

@@ -26,14 +26,18 @@ struct ActIn {
     int e4m3, relu, zero_pad;
 };
 
-// How the weight gradient is cut up: windows B of L steps (one tap: all rows as one window), CO co tiles per workgroup, tap groups (the first n_hi take nhi taps, the others nhi - 1), splits of `units` units each.  want =
-// the splits aimed at, at least nsplit
-struct ActPlan { int B, L, co, groups, n_hi, nhi, nsplit, units, want; };
+// How the weight gradient is cut up: windows B of L steps (one tap: all rows as one window), co co tiles per workgroup, tap groups
+// (the first n_hi take nhi taps, the others nhi - 1), splits of `units` units each, gx of them side by side.  want = the splits
+// aimed at, at least nsplit
+struct ActPlan { int B, L, co, groups, n_hi, nhi, nsplit, units, want, gx; };
 #define ACT_UNIT 64   // timesteps of a unit
 #define ACT_WAVES 8   // waves of a workgroup
 // Taps a wave takes at most: with 8 the accumulators of one tile leave too few registers (23 to 71 spilled).  15 taps as
 // 5 + 5 + 5 / as 8 + 7, us: 64 -> 128 channels, 37 x 333: 21.5 / 26.5; 128 x 510: 55.8 / 58.4; 64 -> 64, 128 x 510: 36.0 / 33.8.
 #define ACT_TAPS 7
+
+// Rows that a wave sums in one chain (plan: camal_act.hip)
+#define ACT_CHAIN_ROWS 4096
 
 // Where the sums go, in floats: partial sums [split][tap][co][ci], or with one split the gradient [co][ci][tap] itself
 struct ActOut { int split, tap, co, ci; };

@@ -48,13 +48,13 @@ template <int CO, int NTAP> struct ActTile {
 template <int CO, int NTAP>
 __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float* __restrict__ dz, const ActIn& in,
                                                float* __restrict__ part, ActOut out, int B, int L, int cin, int cout,
-                                               int ks, int units_per_split, int j0) {
+                                               int ks, int units_per_split, int split, int z, int j0) {
     using T = ActTile<CO, NTAP>;
     constexpr int WK = T::WK;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave / CO, col = wave % CO;
-    const int i = lane & 31, h = lane >> 5, co0 = (blockIdx.z * CO + col) * 32, ci0 = blockIdx.y % (cin / 32) * 32;
+    const int i = lane & 31, h = lane >> 5, co0 = (z * CO + col) * 32, ci0 = blockIdx.y % (cin / 32) * 32;
     const int tpw = (L + ACT_UNIT - 1) / ACT_UNIT, total = B * tpw;
-    const int lo = min(total, (int)blockIdx.x * units_per_split), hi = min(total, lo + units_per_split);
+    const int lo = min(total, split * units_per_split), hi = min(total, lo + units_per_split);
 
     f32x16 acc[NTAP];
 #pragma unroll
@@ -253,7 +253,7 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
             if (owner == wk)
 #pragma unroll
                 for (int n = n0; n < n0 + CHUNK && n < NTAP; ++n) {
-                    float* po = part + (size_t)blockIdx.x * out.split + (j0 + n) * out.tap + (co0 + 4 * h) * out.co + (ci0 + i) * out.ci;
+                    float* po = part + (size_t)split * out.split + (j0 + n) * out.tap + (co0 + 4 * h) * out.co + (ci0 + i) * out.ci;
 #pragma unroll
                     for (int k = 0; k < OWN / V; ++k) {
                         fv v;
@@ -272,7 +272,7 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
     }
 }
 
-// grid = (splits, tap groups x ci tiles, groups of CO co tiles); the first n_hi tap groups take NHI taps, the others NHI - 1
+// grid = (splits side by side, tap groups x ci tiles, sets of splits x groups of CO co tiles); the first n_hi tap groups take NHI taps, the others NHI - 1
 template <int CO, int NHI>
 __global__ __launch_bounds__(64 * ACT_WAVES, 2) void act_wgrad_kernel(const float* __restrict__ dz, ActIn in, float* __restrict__ part,
                                                                       ActOut out, float* __restrict__ bias_grad, int B, int L,
@@ -280,13 +280,13 @@ __global__ __launch_bounds__(64 * ACT_WAVES, 2) void act_wgrad_kernel(const floa
                                                                       int n_hi) {
     using T = ActTile<CO, NHI>;
     __shared__ __align__(16) unsigned short lds[T::BYTES / 2];
-    const int y = blockIdx.y / (cin / 32);
+    const int y = blockIdx.y / (cin / 32), nz = cout / (32 * CO), z = blockIdx.z % nz, split = blockIdx.z / nz * gridDim.x + blockIdx.x;
     if (bias_grad && blockIdx.x + blockIdx.y + blockIdx.z == 0 && threadIdx.x < cout) bias_grad[threadIdx.x] = 0.f;
     if (y < n_hi) {
-        act_wgrad_body<CO, NHI>(lds, dz, in, part, out, B, L, cin, cout, ks, units_per_split, y * NHI);
+        act_wgrad_body<CO, NHI>(lds, dz, in, part, out, B, L, cin, cout, ks, units_per_split, split, z, y * NHI);
     } else {
         if constexpr (NHI > 1)
-            act_wgrad_body<CO, NHI - 1>(lds, dz, in, part, out, B, L, cin, cout, ks, units_per_split, n_hi * NHI + (y - n_hi) * (NHI - 1));
+            act_wgrad_body<CO, NHI - 1>(lds, dz, in, part, out, B, L, cin, cout, ks, units_per_split, split, z, n_hi * NHI + (y - n_hi) * (NHI - 1));
     }
 }
 
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(64 * ACT_WAVES, 2) void act_wgrad_kernel(const floa
 template <int CO>
 int act_wgrad_launch(hipStream_t s, const ActPlan& p, const float* dz, const ActIn& in, float* sums, ActOut out, float* bias_grad, int cin,
                      int cout, int ks) {
-    const dim3 grid(p.nsplit, p.groups * (cin / 32), cout / (32 * CO));
+    const dim3 grid(p.gx, p.groups * (cin / 32), p.nsplit / p.gx * (cout / (32 * CO)));
     auto launch = [&](auto taps) {
         hipLaunchKernelGGL((act_wgrad_kernel<CO, decltype(taps)::value>), grid, dim3(64 * ACT_WAVES), 0, s, dz, in, sums, out, bias_grad,
                            p.B, p.L, cin, cout, ks, p.units, p.n_hi);

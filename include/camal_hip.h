@@ -254,7 +254,8 @@ size_t camal_trainer_running_count_widths(int mid_channels);                    
 /* The same with 8-bit activation checkpoints (below): act_format CAMAL_ACT_INT8 or CAMAL_ACT_E4M3 keeps the forward pass for
  * the backward pass in one byte per element, CAMAL_ACT_NONE in fp32 (the calls above).  The forward pass, the loss and the
  * ReLU masks are the same bit for bit (but a NaN passes the ReLU here); the gradients see the normalised activations as the codes hold them.  With
- * mid_channels 64 a timestep takes 3.8 KB of workspace instead of 11.1 KB.                                       */
+ * mid_channels 64 a timestep takes 3.8 KB of workspace instead of 11.1 KB (batches of more than about a million timesteps: up
+ * to 0.3 KB more for the weight gradient's partial sums).                                                        */
 #define CAMAL_ACT_NONE (-1)
 #define CAMAL_ACT_INT8 0
 #define CAMAL_ACT_E4M3 1
@@ -365,7 +366,8 @@ int camal_act_norm_bwd(const float* da_dev, int pooled, const void* codes_dev, c
  *   a = bf16([relu](fma(x, gamma, beta)) [+ fma(x_r, gamma_r, beta_r)])
  * The activation enters with the 8 significant bits of bf16 (its code has at most 7); dz enters with all of its 24 and
  * the products are summed in fp32.  dz_dev [B][L][cout] fp32, dw [cout][cin][ks] fp32.  cin, cout in {32, 64, 128, 256},
- * ks <= 63.  An infinite dz gives NaN; a NaN in the input may reach every tap of its channel.                      */
+ * ks <= 63.  An infinite dz gives NaN; a NaN in the input may reach every tap of its channel.  Partial sums of some 4096 rows
+ * each are added up at the end: the workspace grows with B * L, the error does not.                                */
 size_t camal_act_wgrad_workspace_bytes(int B, int L, int cin, int cout, int ks); /* 0 if unsupported */
 int camal_act_wgrad(const float* dz_dev, const void* codes_dev, const unsigned char* scales_dev, int format, int B, int L, int cin,
                     int cout, int ks, const float* gamma, const float* beta, int relu, const void* codes_r_dev,

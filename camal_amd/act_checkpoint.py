@@ -194,7 +194,7 @@ def conv_weight_grad(dz, ckpt, kernel_size, gamma, beta, relu=True, skip=None, z
     if not torch.is_tensor(dz) or dz.dim() != 3 or dz.shape[-1] not in CHANNELS:
         raise ValueError(f"dz is [windows, time, channels] with channels in {CHANNELS}")
     cout, ks = dz.shape[-1], int(kernel_size)
-    if not 1 <= ks <= 63 or ks % 2 == 0:
+    if ks != kernel_size or not 1 <= ks <= 63 or ks % 2 == 0:
         raise _lib.CamalHipError("kernel_size must be odd and in 1..63")
     dz = _floats(dz, (B, L, cout), dev, "dz")
     g, b = _floats(gamma, (cin,), dev, "gamma"), _floats(beta, (cin,), dev, "beta")

@@ -541,3 +541,15 @@ def test_device_refusals():
             ac.conv_weight_grad(dz, ckpt, ks, *n[2:])
     with pytest.raises(_lib.CamalHipError):
         ac.write(z[:, :0], *n)
+
+
+@gpu
+def test_kernel_size_is_a_whole_number():
+    from camal_amd import _lib
+    from camal_amd import act_checkpoint as ac
+    (z, _), n, _, _, dz = _inputs(1, 9, 64, 32)
+    _, ckpt = ac.write(z, *n)
+    for ks in (3.5, 1.25, 7.999):
+        with pytest.raises(_lib.CamalHipError):
+            ac.conv_weight_grad(dz, ckpt, ks, *n[2:])
+    assert torch.equal(ac.conv_weight_grad(dz, ckpt, 3.0, *n[2:]), ac.conv_weight_grad(dz, ckpt, 3, *n[2:]))

@@ -238,8 +238,11 @@ ActIn t_kept_input(const camal_trainer* t, const float* params, int li);
 // gradient is zero; torch's value is rounding noise of sum(dz)).
 // `li`: the layer reads what conv layer li reads
 int t_wgrad(camal_trainer* t, hipStream_t s, const TLayer& l, int li, const float* params, const float* dz, float* grads, int B, int L) {
-    if (t->ckpt())
+    if (t->ckpt()) {
+        if (act_wgrad_bytes(B, L, l.cin, l.cout, l.ks) > t->wg_part_floats * sizeof(float))
+            return fail(CAMAL_ERR_STATE, "wgrad partial buffer too small");
         return act_wgrad(s, dz, t_kept_input(t, params, li), B, L, l.cin, l.cout, l.ks, grads + l.w, grads + l.b, t->wg_part);
+    }
     const float* ain = t->act[li - 1];
     int wps = 1;  // tiles per split
     const int nsplit = wgrad_splits(t, l, B, L, &wps);

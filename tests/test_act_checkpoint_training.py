@@ -273,3 +273,27 @@ def test_one_forward_pass_serves_several_backward_passes(fmt, mid, B, L):
     eng.forward_backward(x, y, update_running=False)  # a whole step is a forward pass, too
     assert torch.equal(backward(losses[0])[0], own[0][0])
     eng.close()
+
+
+@gpu
+@pytest.mark.parametrize("k,mid", [(25, 32), (7, 64)])
+def test_long_batches_on_a_longer_workspace(k, mid):
+    """Batches of over a million timesteps, whose weight gradients are summed in several sets: a shorter batch on the workspace
+    of a longer one gives what it gives on its own, bit for bit."""
+    from camal_amd import synth
+    from camal_amd.trainer import TrainEngine
+    if torch.cuda.mem_get_info()[0] < 32 << 30:
+        pytest.skip("needs 32 GB of GPU memory")
+    m = _model(k, "camal", mid)
+    big = TrainEngine(m, "cuda:0", 230, 10080, act_checkpoint="int8")
+    for B, L in ((230, 10080), (113, 10080), (229, 9970)):
+        g = torch.Generator(device="cuda").manual_seed(B)
+        x = torch.randn(B, L, device="cuda", generator=g)
+        y = (torch.arange(B, device="cuda") % 2).to(torch.int32)
+        own = TrainEngine(m, "cuda:0", B, L, act_checkpoint="int8")
+        big.forward_backward(x, y)
+        own.forward_backward(x, y)
+        assert torch.isfinite(own.grads).all() and own.grads.abs().max() > 0
+        assert torch.equal(big.grads, own.grads), (B, L)
+        own.close()
+    big.close()

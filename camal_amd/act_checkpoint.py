@@ -9,7 +9,8 @@ BatchNorm + ReLU backward (``norm_backward``) and the weight gradient of the lay
 steps on them.
 
 Tensors are ``[window, time, channel]`` on one GPU, channels in {32, 64, 128, 256}; the calls are asynchronous on the
-current stream of that GPU.
+current stream of that GPU.  They are the parts of a backward pass written out by hand: none of them is recorded by autograd,
+whatever requires a gradient among its arguments, and what they return does not require one.
 """
 from __future__ import annotations
 
@@ -27,7 +28,8 @@ FORMATS = {"int8": (torch.int8, _lib.ACT_INT8), "e4m3": (torch.float8_e4m3fn, _l
 @dataclass(frozen=True)
 class ActivationCheckpoint:
     """``codes`` [B, L, C] (``torch.int8`` or ``torch.float8_e4m3fn``) and ``scales`` [B, L, C / 32] (``torch.uint8``):
-    the normalised value of an element is ``code * 2 ** (scale - 127)``."""
+    the normalised value of an element is ``code * 2 ** (scale - 127)``, scales from 1 on; 255 goes with codes 0 and makes the
+    block's values NaN."""
     codes: torch.Tensor
     scales: torch.Tensor
 

@@ -92,7 +92,7 @@ int act_norm_bwd_impl(hipStream_t s, const float* da, ActCodes k, const float* i
 // A long call gets gx of them at a time, one set after the other (the tiles of a set read the same rows), so that a wave's chain of
 // fp32 sums stays near ACT_CHAIN_ROWS rows: twice that at most, where long and short units alternate.  A matrix product cuts its
 // sum off instead of rounding it, an error of one sign that grows with the chain: dz and input of one sign, 100 x 10080, 256 -> 256
-// channels, 63 taps 1.3e-4 in one chain and 2.6e-6 here (a plain fp32 product 2.0e-6).  us, one set of longer chains / sets of
+// channels, 63 taps 1.3e-4 in two chains and 2.6e-6 here (a plain fp32 product 2.0e-6).  us, one set of longer chains / sets of
 // 8192 / 4096 rows: that case 24600 / 17430 / 17840 (one set leaves CUs idle); 7 taps, 400 x 10080, 128 -> 128: 1957 / 2024 / 2064;
 // 3 taps, 800 x 10080, 256 -> 256: 9480 / 9260 / 9330.
 // CO = co tiles of a workgroup, as many as there are up to 4: they share the decoding of their input.  (Two of four tiles leave

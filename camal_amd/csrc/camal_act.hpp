@@ -32,8 +32,8 @@ struct ActIn {
 struct ActPlan { int B, L, co, groups, n_hi, nhi, nsplit, units, want, gx; };
 #define ACT_UNIT 64   // timesteps of a unit
 #define ACT_WAVES 8   // waves of a workgroup
-// Taps a wave takes at most: with 8 the accumulators of one tile leave too few registers (23 to 71 spilled).  15 taps as
-// 5 + 5 + 5 / as 8 + 7, us: 64 -> 128 channels, 37 x 333: 21.5 / 26.5; 128 x 510: 55.8 / 58.4; 64 -> 64, 128 x 510: 36.0 / 33.8.
+// Taps a wave takes at most.  With 8 their accumulators leave too few registers for the rest: 23 to 71 spilled, with 7 none, 8 or
+// 26 (four, two, one co tile).  15 taps as 5 + 5 + 5 / as 8 + 7, us: 64 -> 128 channels, 37 x 333: 21.5 / 26.5; 128 x 510: 55.8 / 58.4; 64 -> 64, 128 x 510: 36.0 / 33.8.
 #define ACT_TAPS 7
 
 // Rows that a wave sums in one chain (plan: camal_act.hip)

@@ -260,9 +260,14 @@ __global__ __launch_bounds__(ACT_FINAL_THREADS) void act_bwd_final_kernel(const 
     dgamma[c] = (float)b;
 }
 
-// A dz that the 256 MiB L3 cannot hold for its reader is stored past it (STREAM): left there, its lines are written out under
-// the next kernel's reads.  24 x 10080 x 256 (248 MB): 179 -> 150 us, all of it in the first stage's reads.  The same stores in
-// the write and read kernels change nothing (83.0 and 47.3 us either way on 124 and 189 MB).
+// From half the 256 MiB L3 on, dz is stored past it (STREAM): left there, its lines push out what the next kernels read and are
+// written out under their reads.  us of 128 channels and dz of 140 / 180 / 220 / 300 / 500 MiB, kept in the L3 -> stored past it:
+//   the call alone                       104 -> 88   132 -> 109   163 -> 134   226 -> 195   377 -> 350
+//   with a 1-tap weight gradient of dz   157 -> 147  201 -> 185   249 -> 229   336 -> 320   559 -> 552
+//   with a 3-tap one                     182 -> 177  230 -> 224   281 -> 275   383 -> 382   639 -> 646
+//   with an elementwise pass over dz     135 -> 141  186 -> 182   235 -> 228   330 -> 325   558 -> 556
+// so its reader gains, too, but for an elementwise one at the lower end.  The same stores in the write and read kernels change
+// nothing (83.0 and 47.3 us either way on 124 and 189 MB).
 #define ACT_STREAM_BYTES (128u << 20)
 template <bool STREAM>
 __device__ __forceinline__ void act_store4(float* p, const float (&o)[4]) {  // (a run-time choice: hipcc merges the two stores)
@@ -299,7 +304,7 @@ __global__ __launch_bounds__(256) void act_bwd_apply_kernel(const float* __restr
 // All of it in one launch for at most ACT_SMALL_ROWS rows, where three launches cost more than the work: a workgroup has 32
 // channels (a scale block) and keeps its rows in registers between the sums and their use.  A call in a stream of calls /
 // alone: 14.7 / 28.1 us here and 19.5 / 31.2 us there at 384 rows, 14.8 / 30.7 at 1024, 15.8 / 38.2 at 2048 (32 to 256
-// channels alike).
+// channels alike).  fp32 sums run over the at most 8 rows of a lane and are then carried in 64 bits.
 #define ACT_SMALL_ROWS 1024
 template <typename F, bool RELU, bool BCAST>
 __global__ __launch_bounds__(1024) void act_bwd_small_kernel(const float* __restrict__ da, const unsigned* __restrict__ codes,

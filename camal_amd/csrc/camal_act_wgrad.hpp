@@ -12,9 +12,11 @@ namespace camal {
 //   dw[co][ci][j] = sum_{b,t} dz[b][t][co] a[b][clamp(t + j - ks/2)][ci],  a = bf16(relu(gamma x + beta) [+ skip])
 // GEMM view: M = co, N = ci, K = time, for every tap j.  v_mfma_f32_32x32x16_bf16 takes 16 timesteps per instruction: lane
 // (i = l & 31, h = l >> 5) feeds 8 consecutive times of channel co_i (A) and ci_i (B).
-//   a holds 8 significant bits (the code behind it has 7 or 4), so it is a bf16 operand without loss.  dz is cut into three
-//   bf16 pieces, each the leading 8 bits of what is left: they add up to it exactly, so the three products, summed in the
-//   instruction's fp32, are an fp32 product sum at a third of the bf16 rate, 5 times the rate of fp32 MFMA.
+//   A code and its scale are exact in bf16, the activation made of them is not: it is computed in fp32 and rounded to bf16, by at
+//   most 2^-8 of itself.  dz is cut into three bf16 pieces, each the leading 8 bits of what is
+//   left: they add up to it exactly, so the three products, summed in the instruction's fp32, are an fp32 product sum of dz and
+//   the rounded activation at a third of the bf16 rate, 5 times the rate of fp32 MFMA.  (Pieces and products below 2^-126 count
+//   as zero: a dz under about 2^-104 keeps fewer of its bits.)
 // One wave = 32 co x 32 ci x NTAP taps on a unit of 64 timesteps.  The 8 waves of a workgroup are CO co tiles x WK units:
 // the CO waves of a unit share its decoded input, and the WK sums of a tile are added in LDS before they leave the workgroup
 // (what the partial sums weigh is what bounds a short call).
@@ -25,12 +27,17 @@ namespace camal {
 //      has bank conflicts.
 // On these SIMDs a vector instruction hides behind a matrix product only up to about three per product (measured: 15.9 ns a
 // product alone, 16.3 with 2, 18.1 with 4, 23.3 with 8 vector instructions to each, two waves), so what counts beside the
-// products is the number of vector instructions: cutting dz takes 44 per 21 products of 7 taps, decoding is shared.
+// products is the number of vector instructions: cutting dz takes 44 per 21 products of 7 taps, decoding is shared.  The source
+// deals cutting and decoding out between the products; the compiled loop keeps to that in part only, since format, skip branch
+// and zero padding are run-time choices and each ends a basic block: a step of <4, 7> is 20 products, the decoding (4 + 17 or 4 +
+// 36 vector instructions) without one, 38 to 42 of cutting with one to three in between, and so on.  Registers that find no place,
+// per lane: 4, 12 and 26 with one co tile and 5, 6 and 7 taps, 8 with two and 7, else none.
 // 256 -> 256 channels, 7 taps, 8 x 10080: 173 to 180 us, 1240 to 1290 TF of bf16 products (MFMA busy 0.71, the clock at 1.74 GHz under this load;
 // a large library product reaches 1130 TF here); 128 -> 128, 7 taps, 128 x 510: 43 us (and 6 of the
 // second stage), of which about 7 until the first product,
-// 25 in the products and 6 in writing 29 MB of sums at the end.  With two pieces of dz instead
-// of three: 0.8 of the time, error 2.5e-6 instead of 3e-7 (norm-wise): not taken.
+// 25 in the products and 6 in writing 29 MB of sums at the end.  Error against 64 bits on that case, norm-wise, dz of either sign:
+// 2.7e-7 (8 x 10080 of 256 channels 4.9e-7 to 5.9e-7); with two pieces of dz instead of three 2.5e-6 in 0.8 of the time: not taken.
+// Where all terms have one sign 8e-8 and 1.1e-6, and 2.6e-6 at any length (the chains of sums are bounded: camal_act.hip).
 // Each split's sums go to part[split][j][co][ci]; act_wgrad_reduce_kernel adds them in a fixed order.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -196,8 +203,9 @@ __device__ __forceinline__ void act_wgrad_body(unsigned short* lds, const float*
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 // Between the products of step s: the next step's dz is cut and its registers loaded again, a quarter of the
-                // next tile decoded and its codes fetched again.  In clumps of their own these would leave the matrix pipe
-                // idle (the two waves of a SIMD share it evenly, reach their clumps together and overlap nothing).
+                // next tile decoded and its codes fetched again.  In clumps of their own these leave the matrix pipe idle (the
+                // two waves of a SIMD share it evenly, reach their clumps together and overlap nothing); what the compiler
+                // makes of this order is said above.
                 constexpr int STASH = (T::PASS + 3) / 4, TASKS = 5 + STASH;
 #pragma unroll
                 for (int n = 0; n < NTAP; ++n) {

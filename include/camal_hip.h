@@ -328,7 +328,7 @@ int camal_trainer_peek(camal_trainer* t, int what, int index, int B, int L, floa
  * code * 2^(scale - 127):
  *   CAMAL_ACT_INT8  code = two's complement byte, the scale is the smallest power of two with max|x| <= 127 * 2^(scale-127)
  *   CAMAL_ACT_E4M3  code = OCP e4m3 (4 exponent, 3 fraction bits), max|x| <= 448 * 2^(scale-127)
- * (scale >= 1; 255 with zero codes = the block holds an infinity, a NaN or a magnitude over 127 * 2^121 (int8) or
+ * (scale >= 1, a 0 reads back as zeros; 255 with zero codes = the block holds an infinity, a NaN or a magnitude over 127 * 2^121 (int8) or
  * 448 * 2^119 (e4m3): it reads back as NaN).  x is rounded to the nearest code, ties to even.  With relu, where that code would put fma(value, gamma, beta) on the other side of the
  * ReLU than fma(x, gamma, beta), the neighbour on x's side is taken: the backward pass has the forward pass's mask
  * exactly (gamma and beta must be the ones the checkpoint was written with).
@@ -355,7 +355,7 @@ int camal_act_read(const void* codes_dev, const unsigned char* scales_dev, int f
  *   dy = da * [fma(x, gamma, beta) > 0] (relu != 0; else dy = da),  dbeta = sum dy,  dgamma = sum dy x,
  *   dz = gamma invstd (dy - dbeta / N - x dgamma / N)
  * da_dev [B][L][channels], or with pooled != 0 [B][channels], the gradient of each window's mean over time: every
- * timestep gets da / L.  Sums are held in 64 bits across workgroups.                                              */
+ * timestep gets da / L.  Sums are held in 64 bits but for the up to 16 rows that a lane adds in 32.                */
 size_t camal_act_norm_bwd_workspace_bytes(long long rows, int channels); /* 0 if unsupported */
 int camal_act_norm_bwd(const float* da_dev, int pooled, const void* codes_dev, const unsigned char* scales_dev, int format, int B,
                        int L, int channels, const float* invstd, const float* gamma, const float* beta, int relu, float* dz_dev,
@@ -364,8 +364,8 @@ int camal_act_norm_bwd(const float* da_dev, int pooled, const void* codes_dev, c
 /* Weight gradient of a Conv1d (odd ks; ks = 1: a linear layer) whose input is held as checkpoint(s):
  *   dw[co][ci][j] = sum_{b,t} dz[b][t][co] * a[b][clamp(t + j - ks/2, 0, L-1)][ci]      (zero_pad: 0 outside the window)
  *   a = bf16([relu](fma(x, gamma, beta)) [+ fma(x_r, gamma_r, beta_r)])
- * The activation enters with the 8 significant bits of bf16 (its code has at most 7); dz enters with all of its 24 and
- * the products are summed in fp32.  dz_dev [B][L][cout] fp32, dw [cout][cin][ks] fp32.  cin, cout in {32, 64, 128, 256},
+ * The activation enters rounded to the 8 significant bits of bf16; dz enters with all of its 24 (fewer below about 2^-104)
+ * and the products are summed in fp32.  dz_dev [B][L][cout] fp32, dw [cout][cin][ks] fp32.  cin, cout in {32, 64, 128, 256},
  * ks <= 63.  An infinite dz gives NaN; a NaN in the input may reach every tap of its channel.  Partial sums of some 4096 rows
  * each are added up at the end: the workspace grows with B * L, the error does not.                                */
 size_t camal_act_wgrad_workspace_bytes(int B, int L, int cin, int cout, int ks); /* 0 if unsupported */
